@@ -4,7 +4,8 @@ Importing the package loads the HIP library (``lib/libkvmove.so``) and the torch
 (``lib/libkvmove_torch.so``), which registers ``torch.ops.block_migration_ops.*`` and
 ``torch.ops.swapping_ops.swap`` exactly as DistServe's worker looks them up
 (reference ``distserve/__init__.py:4-16`` loads SwiftTransformer's ``libst_pybinding.so``
-the same way).  There is no CPU fallback: a missing library is an error here, and every
+the same way), and ``torch.ops.kvcache_ops.*``, the operators that fill and read the pools
+(``cache_ops``).  There is no CPU fallback: a missing library is an error here, and every
 op refuses tensors that are not on the GPU.
 """
 import os
@@ -29,6 +30,8 @@ from distserve_amd.block_manager import BlockLocation, BlockManager  # noqa: E40
 from distserve_amd.config import CacheConfig, DisaggParallelConfig, ModelConfig, ParallelConfig  # noqa: E402
 from distserve_amd.request import MigratingRequest, Request, create_request  # noqa: E402
 from distserve_amd.worker import ParaWorker, Worker  # noqa: E402
+from distserve_amd.cache_ops import (  # noqa: E402
+    StepPlan, paged_attention, plan_prompt, plan_step, prompt_attention, quantized_pool_shape, read_kv, write_kv)
 from distserve_amd.handoff import ContextStageLLMEngine, DecodingStageLLMEngine  # noqa: E402
 from distserve_amd.context_stage_scheduler import (  # noqa: E402
     ContextStageFCFSScheduler, ContextStageSchedConfig, get_context_stage_scheduler)
@@ -40,5 +43,6 @@ __all__ = [
     "ParallelConfig", "MigratingRequest", "Request", "create_request", "ParaWorker", "Worker",
     "ContextStageLLMEngine", "DecodingStageLLMEngine", "DecodingStageFCFSScheduler",
     "DecodingStageSchedConfig", "get_decoding_stage_scheduler", "ContextStageFCFSScheduler",
-    "ContextStageSchedConfig", "get_context_stage_scheduler",
+    "ContextStageSchedConfig", "get_context_stage_scheduler", "StepPlan", "plan_step", "plan_prompt", "write_kv",
+    "read_kv", "paged_attention", "prompt_attention", "quantized_pool_shape",
 ]

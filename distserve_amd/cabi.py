@@ -31,7 +31,14 @@ EXPORTS = (
     "kvm_version", "kvm_last_error", "kvm_get_mem_handle", "kvm_register_mem_handle",
     "kvm_register_source", "kvm_reset", "kvm_opened_handles", "kvm_migrate", "kvm_swap", "kvm_copy_plain",
     "kvm_set_option", "kvm_get_option", "kvm_migrate_plan", "kvm_swap_plan", "kvm_debug_divide",
+    "kvm_plan_words", "kvm_plan_step", "kvm_write_kv", "kvm_read_kv", "kvm_attention_workspace",
+    "kvm_paged_attention", "kvm_prompt_attention",
 )
+
+# element types and pool formats of the cache operators
+KVM_F16, KVM_BF16, KVM_F32 = 0, 1, 2
+KVM_CACHE_PLAIN, KVM_CACHE_E4M3 = 0, 1
+KVM_MAX_HEAD_DIM = 256
 
 
 class KvmError(RuntimeError):
@@ -49,6 +56,29 @@ class KvmGeom(ctypes.Structure):
         ("dec_pp_rank", ctypes.c_int32), ("dec_tp_rank", ctypes.c_int32),
         ("ctx_instance", ctypes.c_int64),
     ]
+
+
+class KvmStep(ctypes.Structure):
+    """What a step plan says about itself (filled by ``plan_step``)."""
+
+    _fields_ = [(name, ctypes.c_int64) for name in (
+        "words", "num_seqs", "num_tokens", "num_kv_tokens", "num_pages", "num_blocks", "block_size", "num_heads",
+        "num_kv_heads", "head_dim", "all_new", "dtype", "row_tiles", "num_row_items", "num_joins", "join_rows",
+        "part_rows", "table_at", "slots_at", "pages_at", "row_items_at", "joins_at")] + [("seal", ctypes.c_uint64)]
+
+
+class KvmCache(ctypes.Structure):
+    """One layer of a K/V pool pair."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + [(name, ctypes.c_int64) for name in (
+        "num_blocks", "num_layers", "layer", "num_kv_heads", "block_size", "head_dim")] + [
+        ("dtype", ctypes.c_int32), ("format", ctypes.c_int32)]
+
+
+class KvmRows(ctypes.Structure):
+    """Rows [tokens][heads][head_dim] by base pointer and strides in elements."""
+
+    _fields_ = [("ptr", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
 
 
 def _lib_path() -> str:
@@ -84,10 +114,21 @@ def _load(path: str) -> ctypes.CDLL:
     lib.kvm_swap_plan.argtypes = [ip, ip, i64, i64, ctypes.c_int, i64, i64, ip]
     lib.kvm_debug_divide.argtypes = [ctypes.c_uint32, ctypes.c_uint32]
     lib.kvm_debug_divide.restype = ctypes.c_uint32
+    i32p, f32 = ctypes.POINTER(ctypes.c_int32), ctypes.c_float
+    step, cache, rows = ctypes.POINTER(KvmStep), ctypes.POINTER(KvmCache), ctypes.POINTER(KvmRows)
+    lib.kvm_plan_words.argtypes = [i64] * 5
+    lib.kvm_plan_words.restype = i64
+    lib.kvm_plan_step.argtypes = [ip, ip, i64, ip, ip, i64, i64, i64, i64, i64, i32, i32p, i64, step]
+    lib.kvm_write_kv.argtypes = [step, vp, cache, rows, rows, vp]
+    lib.kvm_read_kv.argtypes = [step, vp, cache, vp, vp, vp]
+    lib.kvm_attention_workspace.argtypes = [step]
+    lib.kvm_attention_workspace.restype = i64
+    lib.kvm_paged_attention.argtypes = [step, vp, cache, rows, rows, f32, vp, i64, vp]
+    lib.kvm_prompt_attention.argtypes = [step, vp, rows, rows, rows, rows, f32, vp, i64, vp]
     for name in EXPORTS:
         fn = getattr(lib, name)
         if name not in ("kvm_last_error", "kvm_get_option", "kvm_version", "kvm_debug_divide",
-                        "kvm_opened_handles"):
+                        "kvm_opened_handles", "kvm_plan_words", "kvm_attention_workspace"):
             fn.restype = ctypes.c_int
     return lib
 
@@ -205,6 +246,49 @@ class Binding:
     def debug_divide(self, n: int, d: int) -> int:
         return self.lib.kvm_debug_divide(n, d)
 
+    # ---- cache operators
+
+    def plan_step(self, first_token: Sequence[int], new_tokens: Sequence[int], block_table: Sequence[Sequence[int]],
+                  num_blocks: int, block_size: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: int):
+        """(KvmStep, the plan's words as a ctypes array): the words go to device memory as they are.
+        ``num_blocks == 0``: a plan without a cache, ``block_table`` is ignored."""
+        n = len(first_token)
+        if len(new_tokens) != n or (num_blocks and len(block_table) != n):
+            raise KvmError(KVM_EINVAL, f"{n} first tokens, {len(new_tokens)} lengths and {len(block_table)} block tables")
+        tables = block_table if num_blocks else []
+        flat = [block for table in tables for block in table]
+        room = self.lib.kvm_plan_words(n, max(0, sum(new_tokens)), len(flat), num_heads, num_kv_heads)
+        words = (ctypes.c_int32 * max(room, 64))()
+        step = KvmStep()
+        self._check(self.lib.kvm_plan_step(_arr(first_token), _arr(new_tokens), n, _arr(flat), _arr([len(t) for t in tables]),
+                                           num_blocks, block_size, num_heads, num_kv_heads, head_dim, dtype, words,
+                                           len(words), ctypes.byref(step)))
+        return step, words
+
+    def write_kv(self, step: KvmStep, words: int, cache: KvmCache, k: KvmRows, v: KvmRows, stream: int = 0) -> None:
+        self._check(self.lib.kvm_write_kv(ctypes.byref(step), words, ctypes.byref(cache), ctypes.byref(k),
+                                          ctypes.byref(v), stream))
+
+    def read_kv(self, step: KvmStep, words: int, cache: KvmCache, k_out: int, v_out: int, stream: int = 0) -> None:
+        self._check(self.lib.kvm_read_kv(ctypes.byref(step), words, ctypes.byref(cache), k_out, v_out, stream))
+
+    def attention_workspace(self, step: KvmStep) -> int:
+        need = self.lib.kvm_attention_workspace(ctypes.byref(step))
+        if need < 0:
+            self._check(need)
+        return need
+
+    def paged_attention(self, step: KvmStep, words: int, cache: KvmCache, q: KvmRows, out: KvmRows, scale: float,
+                        workspace: int = 0, workspace_bytes: int = 0, stream: int = 0) -> None:
+        self._check(self.lib.kvm_paged_attention(ctypes.byref(step), words, ctypes.byref(cache), ctypes.byref(q),
+                                                 ctypes.byref(out), scale, workspace, workspace_bytes, stream))
+
+    def prompt_attention(self, step: KvmStep, words: int, q: KvmRows, k: KvmRows, v: KvmRows, out: KvmRows,
+                         scale: float, workspace: int = 0, workspace_bytes: int = 0, stream: int = 0) -> None:
+        self._check(self.lib.kvm_prompt_attention(ctypes.byref(step), words, ctypes.byref(q), ctypes.byref(k),
+                                                  ctypes.byref(v), ctypes.byref(out), scale, workspace,
+                                                  workspace_bytes, stream))
+
 
 default = Binding(_lib_path())
 lib = default.lib
@@ -223,3 +307,9 @@ get_option = default.get_option
 swap_plan = default.swap_plan
 migrate_plan = default.migrate_plan
 debug_divide = default.debug_divide
+plan_step = default.plan_step
+write_kv = default.write_kv
+read_kv = default.read_kv
+attention_workspace = default.attention_workspace
+paged_attention = default.paged_attention
+prompt_attention = default.prompt_attention

@@ -30,10 +30,19 @@ KNOWN_KV_SHAPES = {
 
 
 class CacheConfig:
-    """Block size and swap space (reference config.py:9-29; cpu_swap_space is given in GB)."""
+    """Block size and swap space (reference config.py:9-29; cpu_swap_space is given in GB).
+
+    ``cache_dtype`` (not in the reference): "auto" keeps K and V in the model's type, "e4m3" as
+    8-bit codes with a power-of-two scale for each token and head (``head_dim + 1`` bytes).  Both
+    instances of a deployment must use the same: migration moves blocks as they are."""
 
     def __init__(self, block_size: int, max_num_blocks_per_req: int,
-                 gpu_memory_utilization: float = 0.9, cpu_swap_space: int = 0):
+                 gpu_memory_utilization: float = 0.9, cpu_swap_space: int = 0, cache_dtype: str = "auto"):
+        if cache_dtype not in ("auto", "e4m3"):
+            raise ValueError(f"cache_dtype must be 'auto' or 'e4m3', not {cache_dtype!r}")
+        if cache_dtype == "e4m3" and block_size % 16 != 0:
+            raise ValueError(f"a quantised cache wants a block_size that is a multiple of 16, not {block_size}")
+        self.cache_dtype = cache_dtype
         self.block_size = block_size
         self.max_num_blocks_per_req = max_num_blocks_per_req
         self.gpu_memory_utilization = gpu_memory_utilization
@@ -143,6 +152,14 @@ class ModelConfig:
         if getattr(cfg, "num_key_value_heads", None) is not None:
             return cfg.num_key_value_heads // tp
         total = cfg.num_attention_heads
+        assert total % tp == 0, (
+            f"Total number of attention heads ({total}) must be divisible by the size of "
+            f"tensor parallel group ({tp}).")
+        return total // tp
+
+    def get_num_query_heads(self, parallel_config: ParallelConfig = ParallelConfig()) -> int:
+        """Query heads of one tensor rank (reference config.py:248-257 splits num_attention_heads evenly)."""
+        total, tp = self.hf_config.num_attention_heads, parallel_config.tensor_parallel_size
         assert total % tp == 0, (
             f"Total number of attention heads ({total}) must be divisible by the size of "
             f"tensor parallel group ({tp}).")

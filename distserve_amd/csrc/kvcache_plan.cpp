@@ -1,0 +1,238 @@
+// kvcache_plan.cpp -- the step plan of the cache operators (host only, no device call).
+//
+// A plan is one array of int32 words that the operators' kernels read from device memory:
+//   table   the block tables, one sequence after the other
+//   slots   for each new token, its cache slot (block * block_size + offset)
+//   pages   for each table entry, {first row of the read-back output, tokens in the block}
+//   row items   the attention's work list (KvItem), longest first
+//   joins   which partial rows make up which output rows (KvJoin)
+// Lengths, block ids and the write set are checked while it is built, so no kernel can be
+// sent outside a pool by a plan, and the work list is balanced over the whole batch: long
+// sequences are cut into pieces of the length that spreads the step's keys over the chip.
+#include "kvcache_plan.h"
+#include "kv_internal.h"
+
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+#include <cstring>
+#include <vector>
+
+namespace {
+
+int refuse(int code, const char *fmt, ...)
+{
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    return kvm_internal_error(code, buf);
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Sequences' sums stay in int32 (words of the plan), with room for a tile's overhang.
+constexpr int64_t kMaxTokens = (1ll << 31) - 4096;
+
+}  // namespace
+
+uint64_t kvm_step_seal(const KvmStep &s)
+{
+    // FNV-1a over the fields before the seal: a plan filled by hand or half overwritten is refused
+    uint64_t h = 1469598103934665603ull;
+    const unsigned char *p = (const unsigned char *)&s;
+    for (size_t i = 0; i < offsetof(KvmStep, seal); ++i) h = (h ^ p[i]) * 1099511628211ull;
+    return h;
+}
+
+extern "C" {
+
+int64_t kvm_plan_words(int64_t num_seqs, int64_t num_tokens, int64_t num_pages, int64_t num_heads, int64_t num_kv_heads)
+{
+    if (num_seqs < 0 || num_tokens < 0 || num_pages < 0 || num_heads < 1 || num_kv_heads < 1) return KVM_EINVAL;
+    const int64_t group = std::max<int64_t>(1, num_heads / num_kv_heads);
+    const int64_t tiles = num_seqs + num_tokens * group / 16;            // one at least for each sequence
+    const int64_t items = 2 * tiles + kTargetWorkgroups + 64;            // a cut adds one piece for each piece length
+    return 64 + num_pages * 3 + num_tokens + items * kItemWords + tiles * kJoinWords;
+}
+
+int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t num_seqs, const int64_t *table,
+                  const int64_t *table_len, int64_t num_blocks, int64_t block_size, int64_t num_heads,
+                  int64_t num_kv_heads, int64_t head_dim, int32_t dtype, int32_t *words, int64_t capacity, KvmStep *step)
+{
+    if (!step || !words) return refuse(KVM_EINVAL, "kvm_plan_step: null output");
+    if (num_seqs < 0 || (num_seqs > 0 && (!first_token || !new_tokens)))
+        return refuse(KVM_EINVAL, "kvm_plan_step: bad sequence lists");
+    if (dtype != KVM_F16 && dtype != KVM_BF16 && dtype != KVM_F32)
+        return refuse(KVM_EINVAL, "kvm_plan_step: unknown dtype %d", dtype);
+    if (num_heads < 1 || num_kv_heads < 1 || num_heads % num_kv_heads != 0 || num_heads > (1 << 20))
+        return refuse(KVM_EINVAL, "num_heads (%lld) must be a positive multiple of num_kv_heads (%lld)",
+                      (long long)num_heads, (long long)num_kv_heads);
+    if (head_dim < 16 || head_dim > KVM_MAX_HEAD_DIM || head_dim % 16 != 0)
+        return refuse(KVM_EINVAL, "head_dim is %lld: the cache operators want a multiple of 16 up to %d",
+                      (long long)head_dim, KVM_MAX_HEAD_DIM);
+    const bool cached = num_blocks > 0;
+    if (num_blocks < 0 || num_blocks > INT32_MAX) return refuse(KVM_EINVAL, "bad number of blocks %lld", (long long)num_blocks);
+    if (cached) {
+        if (block_size < 1 || block_size > 65536) return refuse(KVM_EINVAL, "block_size %lld is not in [1, 65536]", (long long)block_size);
+        if (num_blocks * block_size > INT32_MAX)
+            return refuse(KVM_EINVAL, "pools of more than 2^31 token slots are not supported");
+        if (num_seqs > 0 && (!table_len || !table)) return refuse(KVM_EINVAL, "kvm_plan_step: null block table");
+    }
+    const int64_t group = num_heads / num_kv_heads;
+
+    // ---- lengths and tables
+    int64_t tokens = 0, kv_tokens = 0, pages = 0;
+    bool all_new = true;
+    for (int64_t s = 0; s < num_seqs; ++s) {
+        const int64_t a = first_token[s], n = new_tokens[s];
+        if (a < 0 || n < 0 || a > kMaxTokens || n > kMaxTokens)
+            return refuse(KVM_ERANGE, "sequence %lld: first_token %lld, new_tokens %lld", (long long)s, (long long)a, (long long)n);
+        if (a > 0) all_new = false;
+        tokens += n;
+        kv_tokens += a + n;
+        if (cached) {
+            if (table_len[s] < 0) return refuse(KVM_ERANGE, "sequence %lld: negative table length", (long long)s);
+            if (table_len[s] * block_size < a + n)
+                return refuse(KVM_ERANGE, "sequence %lld has %lld tokens but its block table holds %lld blocks of %lld",
+                              (long long)s, (long long)(a + n), (long long)table_len[s], (long long)block_size);
+            pages += table_len[s];
+        }
+        if (tokens * group > kMaxTokens || kv_tokens > kMaxTokens || pages > kMaxTokens / 2)
+            return refuse(KVM_EINVAL, "a step of more than 2^31 rows, cached tokens or blocks is not supported");
+    }
+    if (!cached && !all_new) return refuse(KVM_EINVAL, "a plan without a cache takes new sequences only");
+
+    KvmStep out;
+    memset(&out, 0, sizeof out);
+    out.num_seqs = num_seqs;
+    out.num_tokens = tokens;
+    out.num_kv_tokens = kv_tokens;
+    out.num_pages = pages;
+    out.num_blocks = num_blocks;
+    out.block_size = cached ? block_size : 0;
+    out.num_heads = num_heads;
+    out.num_kv_heads = num_kv_heads;
+    out.head_dim = head_dim;
+    out.all_new = all_new ? 1 : 0;
+    out.dtype = dtype;
+
+    const int64_t slots = cached ? tokens : 0;
+    out.table_at = 0;
+    out.pages_at = (pages + 1) / 2 * 2;
+    out.slots_at = out.pages_at + 2 * pages;
+    out.row_items_at = (out.slots_at + slots + 3) / 4 * 4;
+    if (out.row_items_at > capacity)
+        return refuse(KVM_EINVAL, "kvm_plan_step: %lld words are too few, kvm_plan_words says how many", (long long)capacity);
+
+    if (cached) {
+        std::vector<uint64_t> taken;   // token slots this step writes, one bit each
+        taken.assign((size_t)((num_blocks * block_size + 63) / 64), 0);
+        int64_t at = 0, slot_at = out.slots_at, row = 0;
+        for (int64_t s = 0; s < num_seqs; ++s) {
+            const int64_t kv = first_token[s] + new_tokens[s];
+            for (int64_t p = 0; p < table_len[s]; ++p) {
+                const int64_t block = table[at + p];
+                if (block < 0 || block >= num_blocks)
+                    return refuse(KVM_ERANGE, "block_table[%lld][%lld] = %lld is outside [0, %lld)", (long long)s,
+                                  (long long)p, (long long)block, (long long)num_blocks);
+                words[out.table_at + at + p] = (int32_t)block;
+                const int64_t done = p * block_size, left = kv - done;
+                words[out.pages_at + 2 * (at + p)] = (int32_t)(row + std::min(done, kv));
+                words[out.pages_at + 2 * (at + p) + 1] = (int32_t)std::max<int64_t>(0, std::min(left, block_size));
+            }
+            int64_t page = first_token[s] / block_size, off = first_token[s] % block_size;
+            for (int64_t i = 0; i < new_tokens[s]; ++i) {
+                const int64_t slot = table[at + page] * block_size + off;
+                uint64_t &w = taken[(size_t)(slot >> 6)];
+                const uint64_t bit = 1ull << (slot & 63);
+                if (w & bit)
+                    return refuse(KVM_EDUP, "two tokens of the step go to token %lld of block %lld (sequence %lld)",
+                                  (long long)off, (long long)table[at + page], (long long)s);
+                w |= bit;
+                words[slot_at++] = (int32_t)slot;
+                if (++off == block_size) {
+                    off = 0;
+                    ++page;
+                }
+            }
+            at += table_len[s];
+            row += kv;
+        }
+    }
+
+    // ---- attention work: row tiles, each over the keys its last row may see
+    int64_t most_rows = 0;
+    for (int64_t s = 0; s < num_seqs; ++s) most_rows = std::max(most_rows, new_tokens[s] * group);
+    // two 16-row tiles share the keys that a wave loads, where the registers hold their accumulators
+    out.row_tiles = most_rows > 16 && head_dim <= 128 ? 2 : 1;
+    const int64_t tile_rows = 16 * out.row_tiles;
+
+    int64_t keys = 0;
+    for (int64_t s = 0; s < num_seqs; ++s)
+        for (int64_t r = 0; r < new_tokens[s] * group; r += tile_rows)
+            keys += first_token[s] + (std::min(r + tile_rows, new_tokens[s] * group) - 1) / group + 1;
+    int64_t piece = ceil_div(ceil_div(keys * num_kv_heads, kTargetWorkgroups), kPieceStep) * kPieceStep;
+    piece = std::max<int64_t>(piece, kMinPiece);
+
+    std::vector<KvItem> items;
+    std::vector<KvJoin> joins;
+    int64_t q_start = 0, table_at = 0, part = 0, join_rows = 0;
+    for (int64_t s = 0; s < num_seqs; ++s) {
+        const int64_t rows = new_tokens[s] * group;
+        for (int64_t r = 0; r < rows; r += tile_rows) {
+            const int64_t here = std::min(tile_rows, rows - r);
+            const int64_t end = first_token[s] + (r + here - 1) / group + 1;
+            const int64_t cuts = std::max<int64_t>(1, end / piece + (end % piece > piece / 2 ? 1 : 0));
+            const int64_t len = ceil_div(ceil_div(end, cuts), kPieceStep) * kPieceStep;
+            const int64_t pieces = ceil_div(end, len);
+            KvItem it;
+            it.q_start = (int32_t)q_start;
+            it.rows = (int32_t)rows;
+            it.first = (int32_t)first_token[s];
+            it.table_at = (int32_t)table_at;
+            it.row0 = (int32_t)r;
+            for (int64_t p = 0; p < pieces; ++p) {
+                it.kv_begin = (int32_t)(p * len);
+                it.kv_end = (int32_t)std::min(end, (p + 1) * len);
+                it.part_row = pieces > 1 ? (int32_t)(part + p * here) : -1;
+                items.push_back(it);
+            }
+            if (pieces > 1) {
+                joins.push_back(KvJoin{(int32_t)q_start, (int32_t)r, (int32_t)here, (int32_t)part, (int32_t)here,
+                                       (int32_t)pieces, 0, 0});
+                part += pieces * here;
+                join_rows = std::max(join_rows, here);
+                if (part > kMaxTokens) return refuse(KVM_EINVAL, "a step of more than 2^31 partial rows is not supported");
+            }
+        }
+        q_start += new_tokens[s];
+        if (cached) table_at += table_len[s];
+    }
+    // the longest pieces first, so that the last workgroups to start are short
+    std::stable_sort(items.begin(), items.end(), [](const KvItem &a, const KvItem &b) {
+        return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin;
+    });
+    out.num_row_items = (int64_t)items.size();
+    out.num_joins = (int64_t)joins.size();
+    out.join_rows = join_rows;
+    out.part_rows = part;
+    out.joins_at = out.row_items_at + (int64_t)items.size() * kItemWords;
+    out.words = out.joins_at + (int64_t)joins.size() * kJoinWords;
+    if (out.words > capacity)
+        return refuse(KVM_EINVAL, "kvm_plan_step: %lld words are too few, kvm_plan_words says how many", (long long)capacity);
+    if (!items.empty()) memcpy(words + out.row_items_at, items.data(), items.size() * sizeof(KvItem));
+    if (!joins.empty()) memcpy(words + out.joins_at, joins.data(), joins.size() * sizeof(KvJoin));
+    out.seal = kvm_step_seal(out);
+    *step = out;
+    return KVM_OK;
+}
+
+int64_t kvm_attention_workspace(const KvmStep *step)
+{
+    if (!step || step->seal != kvm_step_seal(*step)) return refuse(KVM_EINVAL, "the step is not one kvm_plan_step made");
+    return step->part_rows * step->num_kv_heads * (step->head_dim + 2) * (int64_t)sizeof(float);
+}
+
+}  // extern "C"

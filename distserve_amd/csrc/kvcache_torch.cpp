@@ -1,0 +1,280 @@
+// kvcache_torch.cpp -- torch op shim of the cache operators.
+//
+// Registers kvcache_ops: the class StepPlan and the ops that take one.  Tensors are checked
+// and reduced to pointers, sizes and strides; the current HIP stream of their device is handed to the
+// C ABI.  A nonzero return code becomes a RuntimeError carrying kvm_last_error().
+//
+// The plan's words are copied to the device on a stream of their own and the copy is waited
+// for, so a plan is complete when its constructor returns: it can be used on any stream
+// afterwards, and in a captured graph (a graph holds the plan's address, so the plan has to
+// live as long as the graph).
+#include "kvmove.h"
+
+#include <c10/hip/HIPGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/custom_class.h>
+#include <torch/library.h>
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <map>
+#include <mutex>
+#include <set>
+#include <vector>
+
+namespace {
+
+void check(int rc, const char *op)
+{
+    TORCH_CHECK(rc == KVM_OK, op, ": ", kvm_last_error(), " (kvmove error ", rc, ")");
+}
+
+int32_t type_code(at::ScalarType t)
+{
+    switch (t) {
+    case at::kHalf: return KVM_F16;
+    case at::kBFloat16: return KVM_BF16;
+    case at::kFloat: return KVM_F32;
+    default: TORCH_CHECK(false, "the cache operators work on float16, bfloat16 and float32, not ", t);
+    }
+}
+
+// The stream that a device's plans are copied on.
+c10::hip::HIPStream copy_stream(c10::DeviceIndex device)
+{
+    static std::mutex mu;
+    static std::map<c10::DeviceIndex, c10::hip::HIPStream> streams;
+    std::lock_guard<std::mutex> lock(mu);
+    auto it = streams.find(device);
+    if (it == streams.end()) it = streams.emplace(device, c10::hip::getStreamFromPool(false, device)).first;
+    return it->second;
+}
+
+struct StepPlan : torch::CustomClassHolder {
+    KvmStep step;
+    at::Tensor words;
+    c10::ScalarType dtype;
+    std::mutex mu;
+    std::set<hipStream_t> seen;   // streams the allocator has been told of
+
+    StepPlan(std::vector<int64_t> first_token, std::vector<int64_t> new_tokens, std::vector<int64_t> table,
+             std::vector<int64_t> table_len, int64_t num_blocks, int64_t block_size, int64_t num_heads,
+             int64_t num_kv_heads, int64_t head_dim, int64_t type, int64_t device)
+        : dtype((c10::ScalarType)type)
+    {
+        TORCH_CHECK(first_token.size() == new_tokens.size(), "StepPlan: ", first_token.size(), " first tokens but ",
+                    new_tokens.size(), " lengths");
+        TORCH_CHECK(num_blocks == 0 || table_len.size() == new_tokens.size(), "StepPlan: ", table_len.size(),
+                    " block tables for ", new_tokens.size(), " sequences");
+        int64_t in_tables = 0, tokens = 0;
+        for (int64_t n : table_len) {
+            TORCH_CHECK(n >= 0 && n <= (int64_t)table.size(), "StepPlan: bad block table length ", n);
+            in_tables += n;
+        }
+        for (int64_t n : new_tokens) {
+            TORCH_CHECK(n >= 0 && n <= INT32_MAX, "StepPlan: a sequence brings ", n, " tokens");
+            tokens += n;
+        }
+        TORCH_CHECK(num_blocks == 0 || in_tables == (int64_t)table.size(), "StepPlan: block tables of ", in_tables,
+                    " blocks but ", table.size(), " entries");
+        TORCH_CHECK(tokens <= INT32_MAX && num_heads >= 1 && num_heads <= (1 << 20) && num_kv_heads >= 1,
+                    "StepPlan: ", tokens, " tokens of ", num_heads, " heads, ", num_kv_heads, " KV heads");
+        TORCH_CHECK(tokens * num_heads <= ((int64_t)1 << 40), "StepPlan: too many rows");
+        std::vector<int32_t> host((size_t)kvm_plan_words((int64_t)new_tokens.size(), tokens, (int64_t)table.size(), num_heads,
+                                                         num_kv_heads));
+        check(kvm_plan_step(first_token.data(), new_tokens.data(), (int64_t)new_tokens.size(), table.data(),
+                            table_len.data(), num_blocks, block_size, num_heads, num_kv_heads, head_dim, type_code(dtype),
+                            host.data(), (int64_t)host.size(), &step),
+              "StepPlan");
+        if (device < 0) return;   // a plan to look at, without a GPU
+        const c10::hip::HIPGuard guard((c10::DeviceIndex)device);
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        TORCH_CHECK(hipStreamIsCapturing(c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream(), &capture) == hipSuccess &&
+                        capture == hipStreamCaptureStatusNone,
+                    "StepPlan: make the plan before the graph capture that uses it");
+        const c10::hip::HIPStream stream = copy_stream((c10::DeviceIndex)device);
+        {
+            // allocated on the copy stream, so that the memory is free there; users are announced by use()
+            const c10::hip::HIPStreamGuard on(stream);
+            words = at::empty({std::max<int64_t>(step.words, 4)}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, device));
+        }
+        TORCH_CHECK(hipMemcpyAsync(words.data_ptr(), host.data(), (size_t)step.words * 4, hipMemcpyHostToDevice, stream.stream()) == hipSuccess &&
+                        hipStreamSynchronize(stream.stream()) == hipSuccess,
+                    "StepPlan: copying the plan to the device failed");
+    }
+
+    // The words for a call on `device`'s current stream; the allocator is told of the stream, so that the
+    // words' memory is not handed out again before the stream's work is done.
+    const int32_t *use(const at::Tensor &like, const char *op, void **stream)
+    {
+        TORCH_CHECK(words.defined(), op, ": the plan was made without a GPU");
+        TORCH_CHECK(like.device() == words.device(), op, ": the plan is on ", words.device(), ", the tensors on ", like.device());
+        const c10::DeviceIndex device = words.device().index();
+        const c10::hip::HIPStream s = c10::hip::getCurrentHIPStream(device);
+        *stream = (void *)s.stream();
+        {
+            std::lock_guard<std::mutex> lock(mu);
+            if (seen.insert(s.stream()).second)
+                words.record_stream(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device).unwrap());
+        }
+        return words.data_ptr<int32_t>();
+    }
+
+    int64_t device_index() const { return words.defined() ? words.device().index() : -1; }
+};
+
+typedef c10::intrusive_ptr<StepPlan> Plan;
+
+void no_grad(const at::Tensor &t, const char *op)
+{
+    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), op, " has no gradient: call it under torch.no_grad()");
+}
+
+// [tokens (or more), heads, head_dim] of the plan's type, heads contiguous inside.
+KvmRows rows(const Plan &plan, const at::Tensor &t, int64_t tokens, int64_t heads, const char *op, const char *name)
+{
+    const KvmStep &s = plan->step;
+    no_grad(t, op);
+    TORCH_CHECK(t.is_cuda(), op, ": ", name, " must live on the GPU");
+    TORCH_CHECK(t.device() == plan->words.device(), op, ": ", name, " is on ", t.device(), ", the plan on ", plan->words.device());
+    TORCH_CHECK(t.scalar_type() == plan->dtype, op, ": ", name, " is ", t.scalar_type(), ", the plan is for ", plan->dtype);
+    TORCH_CHECK(t.dim() == 3 && t.size(0) >= tokens && t.size(1) == heads && t.size(2) == s.head_dim, op, ": ", name,
+                " must be [", tokens, " or more, ", heads, ", ", s.head_dim, "], got ", t.sizes());
+    TORCH_CHECK(t.stride(2) == 1, op, ": ", name, " must be contiguous within a head, its last stride is ", t.stride(2));
+    // a dimension of one has a stride that means nothing
+    return KvmRows{t.data_ptr(), t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0};
+}
+
+KvmCache cache(const Plan &plan, int64_t layer, const at::Tensor &k, const at::Tensor &v, const char *op)
+{
+    const KvmStep &s = plan->step;
+    for (const at::Tensor *t : {&k, &v}) {
+        TORCH_CHECK(t->is_cuda(), op, ": the pools must live on the GPU");
+        TORCH_CHECK(t->dim() == 5 && t->is_contiguous(), op,
+                    ": a pool must be a contiguous [num_blocks, layers, kv_heads, block_size, head_dim]");
+    }
+    TORCH_CHECK(k.sizes() == v.sizes() && k.dtype() == v.dtype() && k.device() == v.device(), op,
+                ": k_cache and v_cache must agree in shape, dtype and device");
+    const bool coded = k.scalar_type() == at::kByte;
+    TORCH_CHECK(coded || k.scalar_type() == plan->dtype, op, ": the pools are ", k.scalar_type(), ", the plan is for ", plan->dtype);
+    TORCH_CHECK(k.size(4) == s.head_dim + (coded ? 1 : 0), op, ": the pools' last dimension is ", k.size(4), ", ",
+                s.head_dim + (coded ? 1 : 0), " expected", coded ? " (head_dim codes and a scale)" : "");
+    return KvmCache{k.data_ptr(), v.data_ptr(), k.size(0), k.size(1), layer, k.size(2), k.size(3), s.head_dim,
+                    type_code(plan->dtype), coded ? KVM_CACHE_E4M3 : KVM_CACHE_PLAIN};
+}
+
+void write_kv(const Plan &plan, int64_t layer, const at::Tensor &k, const at::Tensor &v, const at::Tensor &k_cache,
+              const at::Tensor &v_cache)
+{
+    void *stream;
+    const int32_t *words = plan->use(k_cache, "write_kv", &stream);
+    const KvmCache c = cache(plan, layer, k_cache, v_cache, "write_kv");
+    const KvmStep &s = plan->step;
+    const KvmRows kr = rows(plan, k, s.num_tokens, s.num_kv_heads, "write_kv", "k"),
+                  vr = rows(plan, v, s.num_tokens, s.num_kv_heads, "write_kv", "v");
+    check(kvm_write_kv(&s, words, &c, &kr, &vr, stream), "write_kv");
+}
+
+std::tuple<at::Tensor, at::Tensor> read_kv(const Plan &plan, int64_t layer, const at::Tensor &k_cache, const at::Tensor &v_cache)
+{
+    void *stream;
+    const int32_t *words = plan->use(k_cache, "read_kv", &stream);
+    const KvmCache c = cache(plan, layer, k_cache, v_cache, "read_kv");
+    const KvmStep &s = plan->step;
+    const c10::hip::HIPGuard guard(k_cache.device().index());
+    const auto options = k_cache.options().dtype(plan->dtype);
+    at::Tensor k = at::empty({s.num_kv_tokens, s.num_kv_heads, s.head_dim}, options), v = at::empty_like(k);
+    check(kvm_read_kv(&s, words, &c, k.data_ptr(), v.data_ptr(), stream), "read_kv");
+    return {k, v};
+}
+
+// The output, and zeros in its rows behind the last sequence's when it is a new one.
+at::Tensor output(const Plan &plan, const at::Tensor &q, const std::optional<at::Tensor> &out, const char *op)
+{
+    if (out.has_value()) {
+        TORCH_CHECK(out->sizes() == q.sizes(), op, ": out is ", out->sizes(), ", q is ", q.sizes());
+        return *out;
+    }
+    at::Tensor made = at::empty(q.sizes(), q.options());
+    if (q.size(0) > plan->step.num_tokens) made.narrow(0, plan->step.num_tokens, q.size(0) - plan->step.num_tokens).zero_();
+    return made;
+}
+
+at::Tensor workspace(const Plan &plan, const at::Tensor &q)
+{
+    // from the allocator for each call: a captured graph gets memory of its own
+    return at::empty({kvm_attention_workspace(&plan->step)}, q.options().dtype(at::kByte));
+}
+
+float scale_of(const Plan &plan, std::optional<double> scale)
+{
+    return scale.has_value() ? (float)*scale : (float)(1.0 / std::sqrt((double)plan->step.head_dim));
+}
+
+at::Tensor paged_attention(const Plan &plan, int64_t layer, const at::Tensor &q, const at::Tensor &k_cache,
+                           const at::Tensor &v_cache, std::optional<double> scale, const std::optional<at::Tensor> &out)
+{
+    const char *op = "paged_attention";
+    void *stream;
+    const int32_t *words = plan->use(k_cache, op, &stream);
+    const KvmCache c = cache(plan, layer, k_cache, v_cache, op);
+    const KvmStep &s = plan->step;
+    const KvmRows qr = rows(plan, q, s.num_tokens, s.num_heads, op, "q");
+    const c10::hip::HIPGuard guard(q.device().index());
+    at::Tensor o = output(plan, q, out, op);
+    const KvmRows orows = rows(plan, o, s.num_tokens, s.num_heads, op, "out");
+    const at::Tensor w = workspace(plan, q);
+    check(kvm_paged_attention(&s, words, &c, &qr, &orows, scale_of(plan, scale), w.data_ptr(), w.numel(), stream), op);
+    return o;
+}
+
+at::Tensor prompt_attention(const Plan &plan, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
+                            std::optional<double> scale, const std::optional<at::Tensor> &out)
+{
+    const char *op = "prompt_attention";
+    void *stream;
+    const int32_t *words = plan->use(q, op, &stream);
+    const KvmStep &s = plan->step;
+    const KvmRows qr = rows(plan, q, s.num_tokens, s.num_heads, op, "q"), kr = rows(plan, k, s.num_tokens, s.num_kv_heads, op, "k"),
+                  vr = rows(plan, v, s.num_tokens, s.num_kv_heads, op, "v");
+    const c10::hip::HIPGuard guard(q.device().index());
+    at::Tensor o = output(plan, q, out, op);
+    const KvmRows orows = rows(plan, o, s.num_tokens, s.num_heads, op, "out");
+    const at::Tensor w = workspace(plan, q);
+    check(kvm_prompt_attention(&s, words, &qr, &kr, &vr, &orows, scale_of(plan, scale), w.data_ptr(), w.numel(), stream), op);
+    return o;
+}
+
+}  // namespace
+
+#ifndef KVM_CACHE_NS
+#define KVM_CACHE_NS kvcache_ops
+#endif
+#define KVM_TEXT_(x) #x
+#define KVM_TEXT(x) KVM_TEXT_(x)
+#define KVM_PLAN "__torch__.torch.classes." KVM_TEXT(KVM_CACHE_NS) ".StepPlan plan"
+#define KVM_TORCH_LIBRARY(ns, m) TORCH_LIBRARY(ns, m)
+
+KVM_TORCH_LIBRARY(KVM_CACHE_NS, m)
+{
+    TORCH_CHECK(kvm_version() / 10000 == KVM_ABI_MAJOR, "libkvmove.so is version ", kvm_version(),
+                ", this op library was built for major version ", KVM_ABI_MAJOR);
+    m.class_<StepPlan>("StepPlan")
+        .def(torch::init<std::vector<int64_t>, std::vector<int64_t>, std::vector<int64_t>, std::vector<int64_t>, int64_t,
+                         int64_t, int64_t, int64_t, int64_t, int64_t, int64_t>())
+        .def("num_tokens", [](const Plan &p) { return p->step.num_tokens; })
+        .def("num_kv_tokens", [](const Plan &p) { return p->step.num_kv_tokens; })
+        .def("workspace_bytes", [](const Plan &p) { return kvm_attention_workspace(&p->step); })
+        .def("device_index", [](const Plan &p) { return p->device_index(); });
+    m.def("write_kv(" KVM_PLAN ", int layer, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache) -> ()", write_kv);
+    m.def("read_kv(" KVM_PLAN ", int layer, Tensor k_cache, Tensor v_cache) -> (Tensor, Tensor)", read_kv);
+    m.def("paged_attention(" KVM_PLAN ", int layer, Tensor q, Tensor k_cache, Tensor v_cache, float? scale=None, "
+          "Tensor? out=None) -> Tensor",
+          paged_attention);
+    m.def("prompt_attention(" KVM_PLAN ", Tensor q, Tensor k, Tensor v, float? scale=None, Tensor? out=None) -> Tensor",
+          prompt_attention);
+}

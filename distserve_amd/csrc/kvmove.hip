@@ -12,6 +12,7 @@
 // Reference call sites this stands behind: distserve/worker.py:133-134 (handles),
 // :239-246 (registration), :250-267 (migrate_blocks), :303-311 (swap).
 #include "kvmove.h"
+#include "kv_internal.h"
 
 #include <hip/hip_runtime.h>
 
@@ -1325,9 +1326,22 @@ bool fits_packed(int64_t n_src, int64_t n_dst) { return n_src <= 65536 && n_dst 
 
 // ------------------------------------------------------------------------- C ABI
 
+// the other translation units of the library report their errors through the same thread-local text
+int kvm_internal_error(int code, const char *text)
+{
+    g_err = text;
+    return code;
+}
+
+int kvm_internal_pool(const void *p, uint64_t need, const char *what, int *device)
+{
+    if (int rc = device_of(p, what, device)) return rc;
+    return check_extent(p, need, extent_of(p), what);
+}
+
 extern "C" {
 
-int kvm_version(void) { return KVM_ABI_MAJOR * 10000 + 0 * 100 + 0; }
+int kvm_version(void) { return KVM_ABI_MAJOR * 10000 + 1 * 100 + 0; }
 
 const char *kvm_last_error(void) { return g_err.c_str(); }
 

@@ -23,6 +23,7 @@ from typing import Callable, Dict, List, Optional, Tuple
 
 import torch
 
+from distserve_amd import cache_ops
 from distserve_amd.config import CacheConfig, ModelConfig, ParallelConfig
 from distserve_amd.request import Request
 from distserve_amd.streams import side_streams
@@ -137,15 +138,21 @@ class Worker:
 
     # ---- pools
 
+    @property
+    def cache_is_quantized(self) -> bool:
+        return getattr(self.cache_config, "cache_dtype", "auto") == "e4m3"
+
     def kv_cache_shape(self, num_blocks: int) -> Tuple[int, int, int, int, int]:
-        return (num_blocks,
-                self.model_config.get_num_layers(self.parallel_config),
-                self.model_config.get_num_heads(self.parallel_config),
-                self.cache_config.block_size,
-                self.model_config.get_head_size())
+        shape = (num_blocks,
+                 self.model_config.get_num_layers(self.parallel_config),
+                 self.model_config.get_num_heads(self.parallel_config),
+                 self.cache_config.block_size,
+                 self.model_config.get_head_size())
+        return cache_ops.quantized_pool_shape(shape) if self.cache_is_quantized else shape
 
     def _new_pool(self, num_blocks: int, on_host: bool) -> torch.Tensor:
-        shape, dtype = self.kv_cache_shape(num_blocks), self.model_config.get_torch_dtype()
+        shape = self.kv_cache_shape(num_blocks)
+        dtype = torch.uint8 if self.cache_is_quantized else self.model_config.get_torch_dtype()
         if on_host:
             # pinned, so that the swap copies are asynchronous to the host
             return torch.empty(shape, dtype=dtype, device="cpu", pin_memory=True)
@@ -163,9 +170,11 @@ class Worker:
     def _get_block_size_in_bytes(self, block_size: int, model_config: ModelConfig,
                                  parallel_config: ParallelConfig) -> int:
         """Bytes of one block, K and V together (reference worker.py:136-150)."""
-        per_pool = (model_config.get_num_layers(parallel_config) * model_config.get_num_heads(parallel_config)
-                    * block_size * model_config.get_head_size())
-        return 2 * per_pool * model_config.get_dtype_size()
+        tokens = (model_config.get_num_layers(parallel_config) * model_config.get_num_heads(parallel_config)
+                  * block_size)
+        if self.cache_is_quantized:
+            return 2 * tokens * (model_config.get_head_size() + 1)
+        return 2 * tokens * model_config.get_head_size() * model_config.get_dtype_size()
 
     def _profile_num_available_blocks(self, block_size: int, gpu_memory_utilization: float,
                                       cpu_swap_space: int, model_bytes: int = 0) -> Tuple[int, int]:
@@ -195,6 +204,34 @@ class Worker:
         out = self.forward(input_tokens_batched, first_token_indexes, self.k_cache, self.v_cache, block_table)
         self.execution_time += time.time() - start
         return out
+
+    # ---- what a model's layers do with the pools (the forward's calls, reference worker.py:211-227)
+
+    def plan_step(self, input_lens: List[int], first_token_indexes: List[int],
+                  block_table: List[List[int]]) -> "cache_ops.StepPlan":
+        """The plan of a step over this worker's pools, from what ``step`` gets: how many tokens each
+        request brings, the index of its first one, its block table.  One plan serves all layers."""
+        return cache_ops.plan_step(self.k_cache, input_lens, first_token_indexes, block_table,
+                                   self.model_config.get_num_query_heads(self.parallel_config),
+                                   self.model_config.get_torch_dtype())
+
+    def write_kv(self, plan, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """New tokens' K and V of a (local) layer into their blocks."""
+        cache_ops.write_kv(plan, layer, k, v, self.k_cache, self.v_cache)
+
+    def read_kv(self, plan, layer: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """K and V of all tokens of the plan's requests."""
+        return cache_ops.read_kv(plan, layer, self.k_cache, self.v_cache)
+
+    def paged_attention(self, plan, layer: int, q: torch.Tensor, scale: Optional[float] = None,
+                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """New tokens' attention over the cache of a (local) layer."""
+        return cache_ops.paged_attention(plan, layer, q, self.k_cache, self.v_cache, scale, out)
+
+    def prompt_attention(self, plan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                         scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Causal attention of whole prompts over K and V at hand (no request has earlier tokens)."""
+        return cache_ops.prompt_attention(plan, q, k, v, scale, out)
 
     # ---- migration
 

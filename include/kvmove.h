@@ -1,5 +1,5 @@
 /*
- * kvmove -- C ABI of the MI355X (gfx950) KV-block migration and swap library.
+ * kvmove -- C ABI of the MI355X (gfx950) library of KV-block migration, swap and cache operators.
  *
  * This is the drop-in boundary for the prefill->decode KV movement path of DistServe.
  * Each entry point names the reference call it stands behind (paths relative to the
@@ -251,6 +251,125 @@ int kvm_swap_plan(const int64_t *src_ids, const int64_t *dst_ids, int64_t n, int
  * check that arithmetic against plain division.  Returns UINT32_MAX for d == 0.
  */
 uint32_t kvm_debug_divide(uint32_t n, uint32_t d);
+
+/* ---------------------------------------------------------------------------------------
+ * Cache operators: writing new tokens' K and V into the pools, reading them back, and the
+ * attention that reads the pools.  In the reference all of this happens inside the model
+ * forward that the worker calls with its pools and block table (distserve/worker.py:211-227);
+ * here the same arguments -- the new tokens of each request, the index of each request's
+ * first new token and the block table -- are turned into a step plan once per step, and
+ * every layer's calls take the plan.
+ * ------------------------------------------------------------------------------------- */
+
+/* Element types of rows (q, k, v, out) and of plain pools. */
+#define KVM_F16 0
+#define KVM_BF16 1
+#define KVM_F32 2
+
+/* What a pool holds.  KVM_CACHE_PLAIN: elements of the rows' type,
+ *     [num_blocks, layers_local, kv_heads_local, block_size, head_dim].
+ * KVM_CACHE_E4M3: bytes, [num_blocks, layers_local, kv_heads_local, block_size, head_dim + 1].
+ * Each (block, layer, head) slab holds block_size * head_dim e4m3 codes, token by token, and
+ * then block_size scale bytes, one for each token: byte b stands for 2^(b-127), and a value
+ * is code * 2^(b-127).  A row x is written with the smallest exponent e for which
+ * max|x| <= 448 * 2^e over its finite elements (0 for a row without any but zeros; -126 at
+ * least): code = x * 2^-e rounded to nearest, ties to even; infinities become +-448, NaN
+ * stays NaN.  Because the scale is a power of two, a value costs one rounding (half a step:
+ * 2^-4 of it, or 2^-10 * 2^e among the small ones) and reading it back costs none.
+ * The slabs are whole, so migration and swap move such a pool like any other, with
+ * dtype_bytes = 1 and head_dim + 1 in the place of head_dim. */
+#define KVM_CACHE_PLAIN 0
+#define KVM_CACHE_E4M3 1
+
+/* Limits of the cache operators. */
+#define KVM_MAX_HEAD_DIM 256   /* head_dim: a multiple of 16, at most this */
+
+/* What a step plan says about itself; kvm_plan_step fills it, the operators read it. */
+typedef struct KvmStep {
+    int64_t words;          /* int32 words of the plan */
+    int64_t num_seqs, num_tokens, num_kv_tokens, num_pages;
+    int64_t num_blocks;     /* of the pools the block table names; 0 = a plan without a cache */
+    int64_t block_size, num_heads, num_kv_heads, head_dim;
+    int64_t all_new;        /* 1 when no sequence has tokens before this step's */
+    int64_t dtype;          /* KVM_F16, KVM_BF16 or KVM_F32 */
+    int64_t row_tiles;      /* 16-row tiles of a workgroup of the row kernel */
+    int64_t num_row_items, num_joins, join_rows;
+    int64_t part_rows;      /* partial rows for each KV head */
+    int64_t table_at, slots_at, pages_at, row_items_at, joins_at;   /* sections, in words */
+    uint64_t seal;          /* guards against a plan that was not made by kvm_plan_step */
+} KvmStep;
+
+/* Words that kvm_plan_step may need at most for such a step. */
+int64_t kvm_plan_words(int64_t num_seqs, int64_t num_tokens, int64_t num_pages, int64_t num_heads,
+                       int64_t num_kv_heads);
+
+/*
+ * The plan of a step: sequence s brings new_tokens[s] tokens behind the first_token[s] that
+ * the cache holds already (distserve/worker.py:194-203: input_tokens_batched,
+ * first_token_indexes), and its blocks are the next table_len[s] entries of table.  Rows of
+ * q, k, v and out are the new tokens of all sequences, one sequence after the other.
+ * Everything an operator could trip over is checked here, on the host: block ids against
+ * num_blocks, tables long enough for first_token + new_tokens, and no cache slot written by
+ * two tokens of the step (KVM_EDUP).  num_blocks == 0: a plan without a cache (table and
+ * table_len are not read), for kvm_prompt_attention only.  The words are to be copied to
+ * device memory as they are; they must outlive the operators that use them.
+ * head_dim, num_heads and num_kv_heads are this rank's; num_heads must be a multiple of
+ * num_kv_heads.  Touches no device.
+ */
+int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t num_seqs, const int64_t *table,
+                  const int64_t *table_len, int64_t num_blocks, int64_t block_size, int64_t num_heads,
+                  int64_t num_kv_heads, int64_t head_dim, int32_t dtype, int32_t *words, int64_t capacity,
+                  KvmStep *step);
+
+/* One layer of a pool pair. */
+typedef struct KvmCache {
+    void *k, *v;
+    int64_t num_blocks, num_layers, layer, num_kv_heads, block_size, head_dim;
+    int32_t dtype;    /* of the rows that go in and out; a plain pool's own */
+    int32_t format;   /* KVM_CACHE_PLAIN or KVM_CACHE_E4M3 (block_size a multiple of 16) */
+} KvmCache;
+
+/* Rows [tokens][heads][head_dim]: elements of a head are contiguous, token and head strides
+ * are in elements and multiples of 16 bytes, the base is 16-byte aligned. */
+typedef struct KvmRows {
+    void *ptr;
+    int64_t token_stride, head_stride;
+} KvmRows;
+
+/* K and V of the step's new tokens into the blocks the plan names.  `words` is the device
+ * copy of the plan.  Slots the step does not name are left as they are. */
+int kvm_write_kv(const KvmStep *step, const int32_t *words, const KvmCache *cache, const KvmRows *k,
+                 const KvmRows *v, void *stream);
+
+/* All tokens of the step's sequences (the earlier ones and the new ones), packed one
+ * sequence after the other: k_out and v_out are [num_kv_tokens, num_kv_heads, head_dim],
+ * contiguous, of the plan's type.  Values of a quantised pool beyond the largest KVM_F16
+ * number become that number. */
+int kvm_read_kv(const KvmStep *step, const int32_t *words, const KvmCache *cache, void *k_out, void *v_out,
+                void *stream);
+
+/* Bytes of device workspace kvm_paged_attention / kvm_prompt_attention want (may be 0); the
+ * contents do not matter and nothing is kept in it between calls, but two calls in flight on
+ * different streams (or two captured graphs that replay at the same time) need one each. */
+int64_t kvm_attention_workspace(const KvmStep *step);
+
+/*
+ * Row i of sequence s and query head a attend over tokens 0 .. first_token[s] + i of the
+ * sequence, in the cache, with KV head a / (num_heads / num_kv_heads):
+ *     out = sum_j softmax_j(scale * q.k_j) v_j.
+ * The new tokens' K and V must be in the cache (kvm_write_kv before it on the stream).
+ * Tokens behind the last sequence's in q and out are neither read nor written.  Cache slots
+ * that no row may attend to (blocks' unused tails, later tokens) do not reach the result,
+ * whatever they hold.  Sums, maxima and accumulators are 32-bit.
+ */
+int kvm_paged_attention(const KvmStep *step, const int32_t *words, const KvmCache *cache, const KvmRows *q,
+                        const KvmRows *out, float scale, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* The same where every sequence is new (first_token[s] == 0) and K and V are at hand as rows:
+ * causal attention of packed prompts. */
+int kvm_prompt_attention(const KvmStep *step, const int32_t *words, const KvmRows *q, const KvmRows *k,
+                         const KvmRows *v, const KvmRows *out, float scale, void *workspace,
+                         int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
