@@ -1,7 +1,7 @@
 """Builds the two shared libraries of the package, in-tree, for gfx950.
 
 ``libkvmove.so``        hand-written HIP kernels + the C ABI (``include/kvmove.h``); no torch.  Migration and
-                        swap are ``kvmove.hip``, the cache operators ``kvcache.hip`` and ``kvcache_plan.cpp``.
+                        swap are ``kvmove.hip``, the cache operators ``kvcache*.hip`` and ``kvcache_plan.cpp``.
 ``libkvmove_torch.so``  torch op shim registering ``block_migration_ops`` / ``swapping_ops`` (``kvmove_torch.cpp``)
                         and ``kvcache_ops`` (``kvcache_torch.cpp``).
 ``tests/lib_explore/libkvmove.so``  the HIP library again with ``-DKVM_EXPLORE``: every kernel flavour and the
@@ -71,7 +71,7 @@ def _objects(specs):
         return list(pool.map(lambda spec: _object(*spec), specs))
 
 
-CACHE_UNITS = [("kvcache.hip", "kvcache.o"), ("kvcache_plan.cpp", "kvcache_plan.o")]
+CACHE_UNITS = [("kvcache.hip", "kvcache.o"), ("kvcache_tiles.hip", "kvcache_tiles.o"), ("kvcache_plan.cpp", "kvcache_plan.o")]
 
 
 def build_kvmove(explore: bool = False, cache_objects=None) -> str:

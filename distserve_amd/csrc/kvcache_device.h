@@ -1,0 +1,148 @@
+// kvcache_device.h -- what the cache operators' kernels share: element types, e4m3 codes, division
+// by a number the host knows, and the attention kernels' arguments.
+#ifndef KVCACHE_DEVICE_H
+#define KVCACHE_DEVICE_H
+
+#include "kvcache_plan.h"
+
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+namespace kvc {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// ---- element types
+
+template <typename T> struct Elem;
+template <> struct Elem<_Float16> {
+    typedef f16x4 V4;
+    typedef f16x8 Frag;     // 16 bytes: an operand of a matrix instruction
+    static constexpr uint32_t kExponent = 0x7c007c00u;
+};
+template <> struct Elem<__bf16> {
+    typedef bf16x4 V4;
+    typedef bf16x8 Frag;
+    static constexpr uint32_t kExponent = 0x7f807f80u;
+};
+template <> struct Elem<float> {
+    typedef f32x4 V4;
+    typedef f32x4 Frag;
+    static constexpr uint32_t kExponent = 0x7f800000u;
+};
+
+// Whether one of the word's elements is an infinity or a NaN (its exponent is all ones).
+template <typename T> __device__ inline bool not_finite(uint32_t w)
+{
+    constexpr uint32_t m = Elem<T>::kExponent;
+    if constexpr (sizeof(T) == 4) return (w & m) == m;
+    return (w & m & 0xffffu) == (m & 0xffffu) || (w & m & 0xffff0000u) == (m & 0xffff0000u);
+}
+
+// ---- e4m3 codes with a power-of-two scale for each row
+
+__device__ inline float power_of(uint32_t byte) { return __uint_as_float(byte << 23); }   // 2^(byte-127), byte >= 1
+
+// Four codes as T, times the row's scale: exact (four significant bits), except that a code may
+// have rounded past the largest fp16 number, which it then becomes (byte >= 135 only: 448 * 2^7
+// still fits).
+template <typename T> __device__ inline void decode4(uint32_t codes, float scale, uint32_t out[])
+{
+    if constexpr (std::is_same<T, _Float16>::value) {
+        union { f16x2 h; uint32_t w; } a, b;
+        a.h = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, false);
+        b.h = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, true);
+        if (scale >= 256.0f) {
+            for (uint32_t *w : {&a.w, &b.w}) {
+                if ((*w & 0x7fffu) == 0x7c00u) *w -= 1;
+                if ((*w & 0x7fff0000u) == 0x7c000000u) *w -= 0x10000u;
+            }
+        }
+        out[0] = a.w;
+        out[1] = b.w;
+    } else if constexpr (std::is_same<T, __bf16>::value) {
+        union { bf16x2 h; uint32_t w; } a, b;
+        a.h = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false);
+        b.h = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true);
+        out[0] = a.w;
+        out[1] = b.w;
+    } else {
+        union { f32x2 f; uint32_t w[2]; } a, b;
+        a.f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, scale, false);
+        b.f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, scale, true);
+        out[0] = a.w[0];
+        out[1] = a.w[1];
+        out[2] = b.w[0];
+        out[3] = b.w[1];
+    }
+}
+
+// Two elements of T in a word (one of float) as floats.
+template <typename T> __device__ inline float element(const uint32_t *w, int i)
+{
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    const uint32_t half = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+    if constexpr (std::is_same<T, __bf16>::value) return __uint_as_float(half << 16);
+    union { uint16_t u; _Float16 h; } c;
+    c.u = (uint16_t)half;
+    return (float)c.h;
+}
+
+// ---- division by a number the host knows: n / d for n < 2^31 (the multiplier has 32 bits)
+
+struct Divider {
+    uint32_t magic, shift;
+};
+
+__host__ inline Divider divider(uint32_t d)
+{
+    uint32_t bits = 0;
+    while ((1ull << bits) < d) ++bits;
+    return Divider{(uint32_t)(((1ull << (31 + bits)) + d - 1) / d), 31 + bits};
+}
+
+__device__ inline uint32_t div_by(uint32_t n, Divider d) { return (uint32_t)(((uint64_t)n * d.magic) >> d.shift); }
+
+// ---- the attention kernels' arguments
+
+struct AttnArgs {
+    const KvItem *items;
+    const int32_t *table;
+    const char *q;
+    char *out;
+    const char *k, *v;                        // the pools at the layer, or the packed rows
+    uint64_t q_token, q_head, out_token, out_head;   // bytes
+    uint64_t k_block, k_head, v_block, v_head;       // bytes: block (or token) and head strides
+    uint32_t row_bytes, codes;                // of a token in the pool; B * D
+    uint32_t block_size, heads, group, head_dim;   // heads: KV heads
+    Divider by_block, by_heads, by_group;
+    float scale_log2;                         // |scale| * log2(e): the softmax is taken in powers of two
+    uint32_t q_sign;                          // sign bits of q to turn over (a negative scale)
+    float *part_acc, *part_ml;                // partial rows: [row][kv head][head_dim], and {maximum, sum}
+};
+
+enum { kPlain = 0, kE4m3 = 1, kPacked = 2 };
+
+template <typename V> __device__ inline V as(u32x4 w)
+{
+    union { u32x4 w; V v; } c;
+    c.w = w;
+    return c.v;
+}
+
+// 2^x
+__device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+}  // namespace kvc
+
+#endif  // KVCACHE_DEVICE_H

@@ -4,7 +4,7 @@
 //   table   the block tables, one sequence after the other
 //   slots   for each new token, its cache slot (block * block_size + offset)
 //   pages   for each table entry, {first row of the read-back output, tokens in the block}
-//   row items   the attention's work list (KvItem), longest first
+//   row items, tile items   the attention's work lists (KvItem), longest first
 //   joins   which partial rows make up which output rows (KvJoin)
 // Lengths, block ids and the write set are checked while it is built, so no kernel can be
 // sent outside a pool by a plan, and the work list is balanced over the whole batch: long
@@ -53,7 +53,7 @@ int64_t kvm_plan_words(int64_t num_seqs, int64_t num_tokens, int64_t num_pages, 
     if (num_seqs < 0 || num_tokens < 0 || num_pages < 0 || num_heads < 1 || num_kv_heads < 1) return KVM_EINVAL;
     const int64_t group = std::max<int64_t>(1, num_heads / num_kv_heads);
     const int64_t tiles = num_seqs + num_tokens * group / 16;            // one at least for each sequence
-    const int64_t items = 2 * tiles + kTargetWorkgroups + 64;            // a cut adds one piece for each piece length
+    const int64_t items = 2 * tiles + 2 * kTargetWorkgroups + 64;            // a cut adds one piece for each piece length
     return 64 + num_pages * 3 + num_tokens + items * kItemWords + tiles * kJoinWords;
 }
 
@@ -163,66 +163,80 @@ int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t
     }
 
     // ---- attention work: row tiles, each over the keys its last row may see
+    //
+    // Sequences of many rows go to the tile kernel (16-bit types; its loads want 16 keys in one block),
+    // the others to the row kernel.
+    auto in_tiles = [&](int64_t s) {
+        return dtype != KVM_F32 && new_tokens[s] * group > kFewRows && (!cached || block_size % 16 == 0);
+    };
     int64_t most_rows = 0;
-    for (int64_t s = 0; s < num_seqs; ++s) most_rows = std::max(most_rows, new_tokens[s] * group);
+    for (int64_t s = 0; s < num_seqs; ++s)
+        if (!in_tiles(s)) most_rows = std::max(most_rows, new_tokens[s] * group);
     // two 16-row tiles share the keys that a wave loads, where the registers hold their accumulators
     out.row_tiles = most_rows > 16 && head_dim <= 128 ? 2 : 1;
-    const int64_t tile_rows = 16 * out.row_tiles;
 
-    int64_t keys = 0;
-    for (int64_t s = 0; s < num_seqs; ++s)
-        for (int64_t r = 0; r < new_tokens[s] * group; r += tile_rows)
-            keys += first_token[s] + (std::min(r + tile_rows, new_tokens[s] * group) - 1) / group + 1;
-    int64_t piece = ceil_div(ceil_div(keys * num_kv_heads, kTargetWorkgroups), kPieceStep) * kPieceStep;
-    piece = std::max<int64_t>(piece, kMinPiece);
-
-    std::vector<KvItem> items;
+    int64_t part = 0, join_rows = 0;
+    std::vector<KvItem> items[2];   // few rows, many rows
     std::vector<KvJoin> joins;
-    int64_t q_start = 0, table_at = 0, part = 0, join_rows = 0;
-    for (int64_t s = 0; s < num_seqs; ++s) {
-        const int64_t rows = new_tokens[s] * group;
-        for (int64_t r = 0; r < rows; r += tile_rows) {
-            const int64_t here = std::min(tile_rows, rows - r);
-            const int64_t end = first_token[s] + (r + here - 1) / group + 1;
-            const int64_t cuts = std::max<int64_t>(1, end / piece + (end % piece > piece / 2 ? 1 : 0));
-            const int64_t len = ceil_div(ceil_div(end, cuts), kPieceStep) * kPieceStep;
-            const int64_t pieces = ceil_div(end, len);
-            KvItem it;
-            it.q_start = (int32_t)q_start;
-            it.rows = (int32_t)rows;
-            it.first = (int32_t)first_token[s];
-            it.table_at = (int32_t)table_at;
-            it.row0 = (int32_t)r;
-            for (int64_t p = 0; p < pieces; ++p) {
-                it.kv_begin = (int32_t)(p * len);
-                it.kv_end = (int32_t)std::min(end, (p + 1) * len);
-                it.part_row = pieces > 1 ? (int32_t)(part + p * here) : -1;
-                items.push_back(it);
+    for (int many = 0; many < 2; ++many) {
+        const int64_t tile_rows = many ? kTileRows : 16 * out.row_tiles;
+        const int64_t step_keys = many ? kTileStep : kPieceStep;
+        int64_t keys = 0;
+        for (int64_t s = 0; s < num_seqs; ++s)
+            for (int64_t r = 0; in_tiles(s) == (many != 0) && r < new_tokens[s] * group; r += tile_rows)
+                keys += first_token[s] + (std::min(r + tile_rows, new_tokens[s] * group) - 1) / group + 1;
+        const int64_t piece = std::max<int64_t>(ceil_div(ceil_div(keys * num_kv_heads, kTargetWorkgroups), step_keys) * step_keys,
+                                                many ? kMinTilePiece : kMinPiece);
+        int64_t q_start = 0, table_at = 0;
+        for (int64_t s = 0; s < num_seqs; ++s) {
+            const int64_t rows = new_tokens[s] * group;
+            for (int64_t r = 0; in_tiles(s) == (many != 0) && r < rows; r += tile_rows) {
+                const int64_t here = std::min(tile_rows, rows - r);
+                const int64_t end = first_token[s] + (r + here - 1) / group + 1;
+                const int64_t cuts = std::max<int64_t>(1, end / piece + (end % piece > piece / 2 ? 1 : 0));
+                const int64_t len = ceil_div(ceil_div(end, cuts), step_keys) * step_keys;
+                const int64_t pieces = ceil_div(end, len);
+                KvItem it;
+                it.q_start = (int32_t)q_start;
+                it.rows = (int32_t)rows;
+                it.first = (int32_t)first_token[s];
+                it.table_at = (int32_t)table_at;
+                it.row0 = (int32_t)r;
+                for (int64_t p = 0; p < pieces; ++p) {
+                    it.kv_begin = (int32_t)(p * len);
+                    it.kv_end = (int32_t)std::min(end, (p + 1) * len);
+                    it.part_row = pieces > 1 ? (int32_t)(part + p * here) : -1;
+                    items[many].push_back(it);
+                }
+                if (pieces > 1) {
+                    joins.push_back(KvJoin{(int32_t)q_start, (int32_t)r, (int32_t)here, (int32_t)part, (int32_t)here,
+                                           (int32_t)pieces, 0, 0});
+                    part += pieces * here;
+                    join_rows = std::max(join_rows, here);
+                    if (part > kMaxTokens) return refuse(KVM_EINVAL, "a step of more than 2^31 partial rows is not supported");
+                }
             }
-            if (pieces > 1) {
-                joins.push_back(KvJoin{(int32_t)q_start, (int32_t)r, (int32_t)here, (int32_t)part, (int32_t)here,
-                                       (int32_t)pieces, 0, 0});
-                part += pieces * here;
-                join_rows = std::max(join_rows, here);
-                if (part > kMaxTokens) return refuse(KVM_EINVAL, "a step of more than 2^31 partial rows is not supported");
-            }
+            q_start += new_tokens[s];
+            if (cached) table_at += table_len[s];
         }
-        q_start += new_tokens[s];
-        if (cached) table_at += table_len[s];
+        // the longest pieces first, so that the last workgroups to start are short
+        std::stable_sort(items[many].begin(), items[many].end(), [](const KvItem &a, const KvItem &b) {
+            return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin;
+        });
     }
-    // the longest pieces first, so that the last workgroups to start are short
-    std::stable_sort(items.begin(), items.end(), [](const KvItem &a, const KvItem &b) {
-        return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin;
-    });
-    out.num_row_items = (int64_t)items.size();
+    out.num_row_items = (int64_t)items[0].size();
+    out.num_tile_items = (int64_t)items[1].size();
     out.num_joins = (int64_t)joins.size();
     out.join_rows = join_rows;
     out.part_rows = part;
-    out.joins_at = out.row_items_at + (int64_t)items.size() * kItemWords;
-    out.words = out.joins_at + (int64_t)joins.size() * kJoinWords;
+    out.tile_items_at = out.row_items_at + out.num_row_items * kItemWords;
+    out.joins_at = out.tile_items_at + out.num_tile_items * kItemWords;
+    out.words = out.joins_at + out.num_joins * kJoinWords;
     if (out.words > capacity)
         return refuse(KVM_EINVAL, "kvm_plan_step: %lld words are too few, kvm_plan_words says how many", (long long)capacity);
-    if (!items.empty()) memcpy(words + out.row_items_at, items.data(), items.size() * sizeof(KvItem));
+    for (int many = 0; many < 2; ++many)
+        if (!items[many].empty())
+            memcpy(words + (many ? out.tile_items_at : out.row_items_at), items[many].data(), items[many].size() * sizeof(KvItem));
     if (!joins.empty()) memcpy(words + out.joins_at, joins.data(), joins.size() * sizeof(KvJoin));
     out.seal = kvm_step_seal(out);
     *step = out;

@@ -28,6 +28,10 @@ constexpr int64_t kJoinWords = sizeof(KvJoin) / 4;
 constexpr int64_t kTargetWorkgroups = 1024;   // four for each of the 256 CUs
 constexpr int64_t kPieceStep = 128;           // keys the four waves of a workgroup take in one turn
 constexpr int64_t kMinPiece = 256;
+constexpr int64_t kFewRows = 32;              // up to here a sequence's rows go to the kernel for few rows
+constexpr int64_t kTileRows = 128;            // of a workgroup of the kernel for many rows
+constexpr int64_t kTileStep = 64;             // keys of its tiles
+constexpr int64_t kMinTilePiece = 512;
 
 uint64_t kvm_step_seal(const KvmStep &s);
 

@@ -292,10 +292,11 @@ typedef struct KvmStep {
     int64_t block_size, num_heads, num_kv_heads, head_dim;
     int64_t all_new;        /* 1 when no sequence has tokens before this step's */
     int64_t dtype;          /* KVM_F16, KVM_BF16 or KVM_F32 */
-    int64_t row_tiles;      /* 16-row tiles of a workgroup of the row kernel */
-    int64_t num_row_items, num_joins, join_rows;
+    int64_t row_tiles;      /* 16-row tiles of a workgroup of the kernel for few rows */
+    int64_t num_row_items, num_tile_items;   /* work for the kernel for few rows, for the one for many */
+    int64_t num_joins, join_rows;
     int64_t part_rows;      /* partial rows for each KV head */
-    int64_t table_at, slots_at, pages_at, row_items_at, joins_at;   /* sections, in words */
+    int64_t table_at, slots_at, pages_at, row_items_at, tile_items_at, joins_at;   /* sections, in words */
     uint64_t seal;          /* guards against a plan that was not made by kvm_plan_step */
 } KvmStep;
 

@@ -10,9 +10,9 @@ import cache_reference as ref
 from distserve_amd import cabi
 
 
-def items_of(step, words):
-    at = step.row_items_at
-    return [tuple(words[at + 8 * i:at + 8 * i + 8]) for i in range(step.num_row_items)]
+def items_of(step, words, many):
+    at, n = (step.tile_items_at, step.num_tile_items) if many else (step.row_items_at, step.num_row_items)
+    return [tuple(words[at + 8 * i:at + 8 * i + 8]) for i in range(n)]
 
 
 def plan(first, new, table, num_blocks=64, block_size=16, heads=8, kv_heads=2, head_dim=64, dtype=cabi.KVM_F16):
@@ -54,26 +54,29 @@ def test_the_pieces_of_a_plan_cover_every_row_and_key_once(heads, kv_heads, head
             starts.append(starts[-1] + b)
             table_at.append(table_at[-1] + p)
         rows = {}
-        lengths = []
-        tile = 16 * step.row_tiles
-        for q_start, total, begin, table_start, row0, kv0, kv1, part in items_of(step, words):
-            owners = [s for s in range(n) if starts[s] == q_start and new[s] > 0]
-            assert len(owners) == 1
-            s = owners[0]
-            assert total == new[s] * group and begin == first[s] and table_start == table_at[s]
-            assert 0 <= kv0 < kv1 <= first[s] + new[s] and kv0 % 128 == 0 and row0 % tile == 0
-            rows.setdefault((s, row0), []).append((kv0, kv1, part))
-            lengths.append(kv1 - kv0)
-        assert lengths == sorted(lengths, reverse=True)
+        tile_of = [128 if dtype != cabi.KVM_F32 and m * group > 32 else 16 * step.row_tiles for m in new]
+        for many in (0, 1):
+            lengths = []
+            for q_start, total, begin, table_start, row0, kv0, kv1, part in items_of(step, words, many):
+                owners = [s for s in range(n) if starts[s] == q_start and new[s] > 0]
+                assert len(owners) == 1
+                s = owners[0]
+                assert total == new[s] * group and begin == first[s] and table_start == table_at[s]
+                assert (tile_of[s] == 128) == bool(many)
+                assert 0 <= kv0 < kv1 <= first[s] + new[s] and row0 % tile_of[s] == 0
+                assert kv0 % (64 if many else 128) == 0
+                rows.setdefault((s, row0), []).append((kv0, kv1, part))
+                lengths.append(kv1 - kv0)
+            assert lengths == sorted(lengths, reverse=True)
         joins = {}
         for i in range(step.num_joins):
             q_start, row0, here, part, pitch, pieces, _, _ = words[step.joins_at + 8 * i:step.joins_at + 8 * i + 8]
             joins[q_start, row0] = (here, part, pitch, pieces)
         used = []
         for s in range(n):
-            for row0 in range(0, new[s] * group, tile):
+            for row0 in range(0, new[s] * group, tile_of[s]):
                 pieces = sorted(rows.pop((s, row0)))
-                here = min(tile, new[s] * group - row0)
+                here = min(tile_of[s], new[s] * group - row0)
                 assert pieces[0][0] == 0 and pieces[-1][1] == first[s] + (row0 + here - 1) // group + 1
                 assert all(a[1] == b[0] for a, b in zip(pieces, pieces[1:]))
                 if len(pieces) == 1:

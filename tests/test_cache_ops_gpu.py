@@ -256,11 +256,18 @@ def test_large_and_odd_scores():
 @pytest.mark.parametrize("hq,h,d,new", [(4, 4, 64, 20), (8, 1, 128, 5), (2, 2, 128, 200), (2, 1, 256, 40)])
 def test_later_tokens_do_not_reach_earlier_rows(dtype, value, hq, h, d, new):
     """An infinity or NaN in one new token's K and V: rows before it come out as if it were not there,
-    rows from it on as the formula says."""
+    rows from it on as the formula says.  (As everywhere, within the error that cache_reference derives: a
+    workgroup that meets such a value takes another order of sums than one that does not, and each of
+    the two is that close to the definition.)"""
     say("later", dtype, value, hq, h, d, new)
     first = 37
     case = Case(dtype, "plain", hq, h, d, 16, [first], [new], seed=9)
-    clean = case.attend()
+    case.check(case.attend(), fast=True)
+    want, tol = ref.attention_fast(case.q, case.seqs[0][0], case.seqs[1][0], first, d ** -0.5, dtype)
+
+    def close(got, rows, cols=slice(None)):
+        return ((got.cpu().double()[rows] - want[rows]).abs() <= tol[rows])[:, :, cols].all()
+
     at = first + new // 2
     spots = {at: slice(3, 5), at + 2: slice(0, 1)} if new > 6 else {at: slice(0, 2)}
     for j, cols in spots.items():
@@ -268,20 +275,20 @@ def test_later_tokens_do_not_reach_earlier_rows(dtype, value, hq, h, d, new):
         case.v_cache[p, case.layer, :, off, cols] = value
     out = case.attend()
     rows = new // 2
-    assert torch.equal(out[:rows], clean[:rows])
+    assert close(out, slice(0, rows))
     after = out[rows:].cpu()
     assert not torch.isfinite(after[:, :, spots[at]]).any()
     # columns that hold no such value stay what they were
     untouched = torch.ones(d, dtype=torch.bool)
     for cols in spots.values():
         untouched[cols] = False
-    assert torch.equal(after[:, :, untouched], clean[rows:].cpu()[:, :, untouched])
+    assert close(out, slice(rows, None), untouched)
     for j in spots:
         p, off = case.table[0][j // 16], j % 16
         case.v_cache[p, case.layer, :, off] = 1.0
         case.k_cache[p, case.layer, :, off] = math.nan
     out = case.attend()
-    assert torch.equal(out[:rows], clean[:rows]) and torch.isnan(out[rows:]).all()
+    assert close(out, slice(0, rows)) and torch.isnan(out[rows:]).all()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -290,21 +297,23 @@ def test_prompts_keep_later_infinities_out_of_earlier_rows(dtype, new):
     say("prompt later", dtype, new)
     q, k, v = (rand((new + 7, 2, 64), dtype, i) for i in range(3))
     plan = plan_prompt([new, 7], 2, 2, 64, dtype)
-    clean = prompt_attention(plan, q.cuda(), k.cuda(), v.cuda())
+    parts = [ref.attention_fast(q[a:b], k[a:b], v[a:b], 0, 64 ** -0.5, dtype) for a, b in ((0, new), (new, new + 7))]
+    want, tol = (torch.cat([p[i] for p in parts]) for i in range(2))
     v[new - 2, :, 5] = math.inf
     out = prompt_attention(plan, q.cuda(), k.cuda(), v.cuda())
-    assert torch.equal(out[:new - 2], clean[:new - 2]) and torch.equal(out[new:], clean[new:])
+    good = (out.cpu().double() - want).abs() <= tol
+    assert good[:new - 2].all() and good[new:].all() and good[new - 2:new, :, :5].all() and good[new - 2:new, :, 6:].all()
     assert not torch.isfinite(out[new - 2:new, :, 5]).any()
 
 
 def test_a_quantised_nan_reaches_only_the_rows_that_see_it():
     case = Case(torch.float16, "e4m3", 4, 2, 64, 16, [20], [10], seed=4)
-    clean = case.attend()
+    want, tol = ref.attention(case.q, case.seqs[0][0], case.seqs[1][0], 20, 64 ** -0.5, torch.float16)
     p, off = case.table[0][25 // 16], 25 % 16
     flat = case.v_cache.view(*case.v_cache.shape[:3], 16 * 65)
     flat[p, case.layer, :, off * 64 + 7] = 0x7f
     out = case.attend()
-    assert torch.equal(out[:5], clean[:5])
+    assert ((out.cpu().double() - want).abs() <= tol)[:5].all()
     assert torch.isnan(out[5:, :, 7]).all() and not torch.isnan(out[5:, :, :7]).any()
 
 
