@@ -65,7 +65,7 @@ class KvmStep(ctypes.Structure):
         "words", "num_seqs", "num_tokens", "num_kv_tokens", "num_pages", "num_blocks", "block_size", "num_heads",
         "num_kv_heads", "head_dim", "all_new", "dtype", "row_tiles", "num_row_items", "num_tile_items",
         "num_joins", "join_rows", "part_rows", "table_at", "slots_at", "pages_at", "row_items_at", "tile_items_at",
-        "joins_at")] + [("seal", ctypes.c_uint64)]
+        "joins_at")] + [("seal", ctypes.c_uint64), ("device", ctypes.c_int64)]
 
 
 class KvmCache(ctypes.Structure):
@@ -73,13 +73,14 @@ class KvmCache(ctypes.Structure):
 
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + [(name, ctypes.c_int64) for name in (
         "num_blocks", "num_layers", "layer", "num_kv_heads", "block_size", "head_dim")] + [
-        ("dtype", ctypes.c_int32), ("format", ctypes.c_int32)]
+        ("dtype", ctypes.c_int32), ("format", ctypes.c_int32), ("extent", ctypes.c_int64)]
 
 
 class KvmRows(ctypes.Structure):
     """Rows [tokens][heads][head_dim] by base pointer and strides in elements."""
 
-    _fields_ = [("ptr", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+    _fields_ = [("ptr", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("extent", ctypes.c_int64)]
 
 
 def _lib_path() -> str:
@@ -121,7 +122,7 @@ def _load(path: str) -> ctypes.CDLL:
     lib.kvm_plan_words.restype = i64
     lib.kvm_plan_step.argtypes = [ip, ip, i64, ip, ip, i64, i64, i64, i64, i64, i32, i32p, i64, step]
     lib.kvm_write_kv.argtypes = [step, vp, cache, rows, rows, vp]
-    lib.kvm_read_kv.argtypes = [step, vp, cache, vp, vp, vp]
+    lib.kvm_read_kv.argtypes = [step, vp, cache, rows, rows, vp]
     lib.kvm_attention_workspace.argtypes = [step]
     lib.kvm_attention_workspace.restype = i64
     lib.kvm_paged_attention.argtypes = [step, vp, cache, rows, rows, f32, vp, i64, vp]
@@ -270,8 +271,10 @@ class Binding:
         self._check(self.lib.kvm_write_kv(ctypes.byref(step), words, ctypes.byref(cache), ctypes.byref(k),
                                           ctypes.byref(v), stream))
 
-    def read_kv(self, step: KvmStep, words: int, cache: KvmCache, k_out: int, v_out: int, stream: int = 0) -> None:
-        self._check(self.lib.kvm_read_kv(ctypes.byref(step), words, ctypes.byref(cache), k_out, v_out, stream))
+    def read_kv(self, step: KvmStep, words: int, cache: KvmCache, k_out: KvmRows, v_out: KvmRows,
+                stream: int = 0) -> None:
+        self._check(self.lib.kvm_read_kv(ctypes.byref(step), words, ctypes.byref(cache), ctypes.byref(k_out),
+                                         ctypes.byref(v_out), stream))
 
     def attention_workspace(self, step: KvmStep) -> int:
         need = self.lib.kvm_attention_workspace(ctypes.byref(step))

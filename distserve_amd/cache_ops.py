@@ -32,12 +32,8 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 
-_ops = torch.ops.kvcache_ops
-# the overloads, resolved once: a lookup through torch.ops per call costs microseconds
-_write_op = _ops.write_kv.default
-_read_op = _ops.read_kv.default
-_paged_op = _ops.paged_attention.default
-_prompt_op = _ops.prompt_attention.default
+# ``torch.ops.kvcache_ops.*`` are the same functions with schemas; the plan's methods, which the functions
+# below call, cost a third of their host time.
 StepPlan = torch.classes.kvcache_ops.StepPlan
 
 # torch's numbers of the types (what C++ calls a ScalarType)
@@ -90,13 +86,13 @@ def plan_prompt(input_lens: Sequence[int], num_heads: int, num_kv_heads: int, he
 def write_kv(plan: StepPlan, layer: int, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
              v_cache: torch.Tensor) -> None:
     """The step's new K and V rows ``[tokens, kv_heads, head_dim]`` into layer ``layer`` of the pools."""
-    _write_op(plan, layer, k, v, k_cache, v_cache)
+    plan.write_kv(layer, k, v, k_cache, v_cache)
 
 
 def read_kv(plan: StepPlan, layer: int, k_cache: torch.Tensor, v_cache: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """K and V of all tokens of the step's sequences, earlier and new, ``[kv_tokens, kv_heads, head_dim]``
     each, one sequence after the other."""
-    return _read_op(plan, layer, k_cache, v_cache)
+    return plan.read_kv(layer, k_cache, v_cache)
 
 
 def paged_attention(plan: StepPlan, layer: int, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -104,10 +100,10 @@ def paged_attention(plan: StepPlan, layer: int, q: torch.Tensor, k_cache: torch.
     """Attention of the step's new tokens ``q`` ``[tokens, heads, head_dim]`` over the cache, each over its
     sequence up to itself; the new tokens' K and V must have been written.  ``scale``: of the scores,
     default ``head_dim ** -0.5``."""
-    return _paged_op(plan, layer, q, k_cache, v_cache, scale, out)
+    return plan.paged_attention(layer, q, k_cache, v_cache, scale, out)
 
 
 def prompt_attention(plan: StepPlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional[float] = None,
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of whole prompts packed one after the other, every sequence of the plan being new."""
-    return _prompt_op(plan, q, k, v, scale, out)
+    return plan.prompt_attention(q, k, v, scale, out)

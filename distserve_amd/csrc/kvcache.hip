@@ -105,7 +105,8 @@ __global__ __launch_bounds__(256) void kvm_read_kernel(const MoveArgs a)
     const uint32_t d = threadIdx.x % LANES * 8;
     if (d >= a.head_dim) return;
     const char *slab = (is_v ? a.src_v : a.src_k) + (uint64_t)block * a.block_stride + head * a.head_stride;
-    char *out = (is_v ? a.dst_v : a.dst_k) + head * a.k_head + d * sizeof(T);
+    const uint64_t token_stride = is_v ? a.v_token : a.k_token;
+    char *out = (is_v ? a.dst_v + head * a.v_head : a.dst_k + head * a.k_head) + d * sizeof(T);
     for (int32_t t = threadIdx.x / LANES; t < count; t += 256 / LANES) {
         uint32_t w[W];
         if constexpr (Q) {
@@ -120,7 +121,7 @@ __global__ __launch_bounds__(256) void kvm_read_kernel(const MoveArgs a)
         }
 #pragma unroll
         for (int i = 0; i < W / 4; ++i)
-            __builtin_nontemporal_store(*(u32x4 *)(w + 4 * i), (u32x4 *)(out + (uint64_t)(first + t) * a.k_token) + i);
+            __builtin_nontemporal_store(*(u32x4 *)(w + 4 * i), (u32x4 *)(out + (uint64_t)(first + t) * token_stride) + i);
     }
 }
 
@@ -200,11 +201,35 @@ int check_launch(const char *what)
 
 int type_bytes(int64_t dtype) { return dtype == KVM_F32 ? 4 : 2; }
 
-int check_step(const KvmStep *step, const int32_t *words, int *device)
+int check_seal(const KvmStep *step)
 {
     if (!step || step->seal != kvm_step_seal(*step)) return refuse(KVM_EINVAL, "the step is not one kvm_plan_step made");
-    if (step->num_tokens == 0) return KVM_OK;
-    return kvm_internal_pool(words, (uint64_t)step->words * 4, "the plan's words", device);
+    return KVM_OK;
+}
+
+// `need` bytes at p, on *device if that is known: by what the caller vouches for, or by asking the runtime.
+int check_memory(const KvmStep *step, const void *p, uint64_t need, int64_t extent, const char *what, int *device)
+{
+    if (!p) return refuse(KVM_EINVAL, "%s is null", what);
+    if (step->device >= 0) {
+        *device = (int)step->device;
+        if (extent < 0 || need > (uint64_t)extent)
+            return refuse(KVM_ERANGE, "%s needs %llu bytes but has %lld", what, (unsigned long long)need, (long long)extent);
+        return KVM_OK;
+    }
+    int dev = -1;
+    if (int rc = kvm_internal_pool(p, need, what, &dev)) return rc;
+    if (*device >= 0 && dev != *device) return refuse(KVM_EINVAL, "%s is on device %d, the plan on device %d", what, dev, *device);
+    *device = dev;
+    return KVM_OK;
+}
+
+int check_words(const KvmStep *step, const int32_t *words, int *device)
+{
+    const uint64_t need = (uint64_t)step->words * 4;
+    *device = -1;
+    if ((uintptr_t)words % 16 != 0) return refuse(KVM_EINVAL, "the plan's words must be 16-byte aligned");
+    return check_memory(step, words, need, (int64_t)need, "the plan's words", device);
 }
 
 struct Layer {
@@ -238,11 +263,8 @@ int check_cache(const KvmStep *step, const KvmCache *c, int device, Layer *out)
     out->head_stride = (uint64_t)c->block_size * (out->row_bytes + (coded ? 1 : 0));
     out->block_stride = out->head_stride * (uint64_t)(c->num_kv_heads * c->num_layers);
     const uint64_t bytes = out->block_stride * (uint64_t)c->num_blocks;
-    int dev = device;
-    KV_TRY(kvm_internal_pool(c->k, bytes, "K pool", &dev));
-    if (dev != device) return refuse(KVM_EINVAL, "the K pool is on device %d, the plan on device %d", dev, device);
-    KV_TRY(kvm_internal_pool(c->v, bytes, "V pool", &dev));
-    if (dev != device) return refuse(KVM_EINVAL, "the V pool is on device %d, the plan on device %d", dev, device);
+    KV_TRY(check_memory(step, c->k, bytes, c->extent, "the K pool", &device));
+    KV_TRY(check_memory(step, c->v, bytes, c->extent, "the V pool", &device));
     const uint64_t layer = out->head_stride * (uint64_t)(c->num_kv_heads * c->layer);
     out->k = (char *)c->k + layer;
     out->v = (char *)c->v + layer;
@@ -258,10 +280,7 @@ int check_rows(const KvmRows *r, const char *what, int64_t tokens, int64_t heads
         return refuse(KVM_EINVAL, "%s: rows must start at multiples of 16 bytes (strides %lld and %lld elements)", what,
                       (long long)r->token_stride, (long long)r->head_stride);
     const uint64_t need = (uint64_t)((tokens - 1) * r->token_stride + (heads - 1) * r->head_stride + step->head_dim) * (uint64_t)size;
-    int dev = device;
-    KV_TRY(kvm_internal_pool(r->ptr, need, what, &dev));
-    if (dev != device) return refuse(KVM_EINVAL, "%s is on device %d, the plan on device %d", what, dev, device);
-    return KVM_OK;
+    return check_memory(step, r->ptr, need, r->extent, what, &device);
 }
 
 // Output rows of different (token, head) must not share memory.
@@ -376,9 +395,7 @@ int attend(const KvmStep *step, const int32_t *words, AttnArgs a, int format, co
         if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16 != 0)
             return refuse(KVM_EINVAL, "the workspace has %lld bytes, %lld (16-byte aligned) are needed",
                           (long long)(workspace ? workspace_bytes : 0), (long long)need);
-        int dev = device;
-        KV_TRY(kvm_internal_pool(workspace, (uint64_t)need, "the workspace", &dev));
-        if (dev != device) return refuse(KVM_EINVAL, "the workspace is on device %d, the plan on device %d", dev, device);
+        KV_TRY(check_memory(step, workspace, (uint64_t)need, workspace_bytes, "the workspace", &device));
     }
     if ((uint64_t)((step->num_row_items + step->num_tile_items) * step->num_kv_heads) > kMaxGroups ||
         (uint64_t)(step->num_joins * step->num_kv_heads) * 16 > kMaxGroups)
@@ -442,8 +459,9 @@ int kvm_write_kv(const KvmStep *step, const int32_t *words, const KvmCache *cach
                  void *stream)
 {
     int device = 0;
-    KV_TRY(check_step(step, words, &device));
+    KV_TRY(check_seal(step));
     if (step->num_tokens == 0) return KVM_OK;
+    KV_TRY(check_words(step, words, &device));
     Layer layer;
     KV_TRY(check_cache(step, cache, device, &layer));
     KV_TRY(check_rows(k, "k", step->num_tokens, step->num_kv_heads, step, device));
@@ -479,17 +497,19 @@ int kvm_write_kv(const KvmStep *step, const int32_t *words, const KvmCache *cach
     return coded ? launch_write_q<float, true>(a, s) : launch_write_q<float, false>(a, s);
 }
 
-int kvm_read_kv(const KvmStep *step, const int32_t *words, const KvmCache *cache, void *k_out, void *v_out, void *stream)
+int kvm_read_kv(const KvmStep *step, const int32_t *words, const KvmCache *cache, const KvmRows *k_out,
+                const KvmRows *v_out, void *stream)
 {
     int device = 0;
-    if (!step || step->seal != kvm_step_seal(*step)) return refuse(KVM_EINVAL, "the step is not one kvm_plan_step made");
+    KV_TRY(check_seal(step));
     if (step->num_kv_tokens == 0) return KVM_OK;
-    KV_TRY(kvm_internal_pool(words, (uint64_t)step->words * 4, "the plan's words", &device));
+    KV_TRY(check_words(step, words, &device));
     Layer layer;
     KV_TRY(check_cache(step, cache, device, &layer));
-    const KvmRows ko = {k_out, step->num_kv_heads * step->head_dim, step->head_dim}, vo = {v_out, ko.token_stride, ko.head_stride};
-    KV_TRY(check_rows(&ko, "k_out", step->num_kv_tokens, step->num_kv_heads, step, device));
-    KV_TRY(check_rows(&vo, "v_out", step->num_kv_tokens, step->num_kv_heads, step, device));
+    KV_TRY(check_rows(k_out, "k_out", step->num_kv_tokens, step->num_kv_heads, step, device));
+    KV_TRY(check_rows(v_out, "v_out", step->num_kv_tokens, step->num_kv_heads, step, device));
+    KV_TRY(check_apart(k_out, "k_out", step->num_kv_tokens, step->num_kv_heads, step->head_dim));
+    KV_TRY(check_apart(v_out, "v_out", step->num_kv_tokens, step->num_kv_heads, step->head_dim));
     if (step->num_pages * step->num_kv_heads > INT32_MAX) return refuse(KVM_EINVAL, "too many blocks for one launch");
     const uint64_t size = (uint64_t)type_bytes(step->dtype);
     MoveArgs a = {};
@@ -497,12 +517,14 @@ int kvm_read_kv(const KvmStep *step, const int32_t *words, const KvmCache *cache
     a.table = words + step->table_at;
     a.src_k = layer.k;
     a.src_v = layer.v;
-    a.dst_k = (char *)k_out;
-    a.dst_v = (char *)v_out;
+    a.dst_k = (char *)k_out->ptr;
+    a.dst_v = (char *)v_out->ptr;
     a.block_stride = layer.block_stride;
     a.head_stride = layer.head_stride;
-    a.k_token = (uint64_t)ko.token_stride * size;
-    a.k_head = (uint64_t)ko.head_stride * size;
+    a.k_token = (uint64_t)k_out->token_stride * size;
+    a.k_head = (uint64_t)k_out->head_stride * size;
+    a.v_token = (uint64_t)v_out->token_stride * size;
+    a.v_head = (uint64_t)v_out->head_stride * size;
     a.row_bytes = layer.row_bytes;
     a.codes = layer.codes;
     a.heads = (uint32_t)step->num_kv_heads;
@@ -523,8 +545,9 @@ int kvm_paged_attention(const KvmStep *step, const int32_t *words, const KvmCach
                         const KvmRows *out, float scale, void *workspace, int64_t workspace_bytes, void *stream)
 {
     int device = 0;
-    KV_TRY(check_step(step, words, &device));
+    KV_TRY(check_seal(step));
     if (step->num_tokens == 0) return KVM_OK;
+    KV_TRY(check_words(step, words, &device));
     Layer layer;
     KV_TRY(check_cache(step, cache, device, &layer));
     AttnArgs a = {};
@@ -542,9 +565,10 @@ int kvm_prompt_attention(const KvmStep *step, const int32_t *words, const KvmRow
                          const KvmRows *out, float scale, void *workspace, int64_t workspace_bytes, void *stream)
 {
     int device = 0;
-    KV_TRY(check_step(step, words, &device));
+    KV_TRY(check_seal(step));
     if (!step->all_new) return refuse(KVM_EINVAL, "prompt attention is for sequences without earlier tokens");
     if (step->num_tokens == 0) return KVM_OK;
+    KV_TRY(check_words(step, words, &device));
     KV_TRY(check_rows(k, "k", step->num_tokens, step->num_kv_heads, step, device));
     KV_TRY(check_rows(v, "v", step->num_tokens, step->num_kv_heads, step, device));
     const uint64_t size = (uint64_t)type_bytes(step->dtype);

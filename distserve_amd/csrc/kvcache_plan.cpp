@@ -39,10 +39,14 @@ constexpr int64_t kMaxTokens = (1ll << 31) - 4096;
 
 uint64_t kvm_step_seal(const KvmStep &s)
 {
-    // FNV-1a over the fields before the seal: a plan filled by hand or half overwritten is refused
-    uint64_t h = 1469598103934665603ull;
-    const unsigned char *p = (const unsigned char *)&s;
-    for (size_t i = 0; i < offsetof(KvmStep, seal); ++i) h = (h ^ p[i]) * 1099511628211ull;
+    // a mix of the words before the seal: a plan filled by hand or half overwritten is refused
+    static_assert(offsetof(KvmStep, seal) % 8 == 0, "the sealed part is whole words");
+    uint64_t h = 0x9e3779b97f4a7c15ull, w;
+    for (size_t i = 0; i < offsetof(KvmStep, seal); i += 8) {
+        memcpy(&w, (const char *)&s + i, 8);
+        h = (h ^ w) * 0xff51afd7ed558ccdull;
+        h ^= h >> 29;
+    }
     return h;
 }
 
@@ -239,6 +243,7 @@ int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t
             memcpy(words + (many ? out.tile_items_at : out.row_items_at), items[many].data(), items[many].size() * sizeof(KvItem));
     if (!joins.empty()) memcpy(words + out.joins_at, joins.data(), joins.size() * sizeof(KvJoin));
     out.seal = kvm_step_seal(out);
+    out.device = -1;
     *step = out;
     return KVM_OK;
 }

@@ -298,6 +298,11 @@ typedef struct KvmStep {
     int64_t part_rows;      /* partial rows for each KV head */
     int64_t table_at, slots_at, pages_at, row_items_at, tile_items_at, joins_at;   /* sections, in words */
     uint64_t seal;          /* guards against a plan that was not made by kvm_plan_step */
+    /* Set by the caller, -1 after kvm_plan_step: the device that the words were copied to, if the caller
+     * vouches that every pointer of its calls with this step lies on that device and for the extents it
+     * gives (a tensor library knows both).  With -1 the operators ask the runtime about every pointer of
+     * every call, about a microsecond each. */
+    int64_t device;
 } KvmStep;
 
 /* Words that kvm_plan_step may need at most for such a step. */
@@ -328,6 +333,7 @@ typedef struct KvmCache {
     int64_t num_blocks, num_layers, layer, num_kv_heads, block_size, head_dim;
     int32_t dtype;    /* of the rows that go in and out; a plain pool's own */
     int32_t format;   /* KVM_CACHE_PLAIN or KVM_CACHE_E4M3 (block_size a multiple of 16) */
+    int64_t extent;   /* bytes from k, and from v, to the end of their memory (step->device >= 0 only) */
 } KvmCache;
 
 /* Rows [tokens][heads][head_dim]: elements of a head are contiguous, token and head strides
@@ -335,6 +341,7 @@ typedef struct KvmCache {
 typedef struct KvmRows {
     void *ptr;
     int64_t token_stride, head_stride;
+    int64_t extent;   /* bytes from ptr to the end of its memory (step->device >= 0 only) */
 } KvmRows;
 
 /* K and V of the step's new tokens into the blocks the plan names.  `words` is the device
@@ -343,11 +350,10 @@ int kvm_write_kv(const KvmStep *step, const int32_t *words, const KvmCache *cach
                  const KvmRows *v, void *stream);
 
 /* All tokens of the step's sequences (the earlier ones and the new ones), packed one
- * sequence after the other: k_out and v_out are [num_kv_tokens, num_kv_heads, head_dim],
- * contiguous, of the plan's type.  Values of a quantised pool beyond the largest KVM_F16
- * number become that number. */
-int kvm_read_kv(const KvmStep *step, const int32_t *words, const KvmCache *cache, void *k_out, void *v_out,
-                void *stream);
+ * sequence after the other: k_out and v_out are [num_kv_tokens, num_kv_heads, head_dim] of the
+ * plan's type.  Values of a quantised pool beyond the largest KVM_F16 number become that number. */
+int kvm_read_kv(const KvmStep *step, const int32_t *words, const KvmCache *cache, const KvmRows *k_out,
+                const KvmRows *v_out, void *stream);
 
 /* Bytes of device workspace kvm_paged_attention / kvm_prompt_attention want (may be 0); the
  * contents do not matter and nothing is kept in it between calls, but two calls in flight on
