@@ -63,9 +63,9 @@ class KvmStep(ctypes.Structure):
 
     _fields_ = [(name, ctypes.c_int64) for name in (
         "words", "num_seqs", "num_tokens", "num_kv_tokens", "num_pages", "num_blocks", "block_size", "num_heads",
-        "num_kv_heads", "head_dim", "all_new", "dtype", "row_tiles", "num_row_items", "num_tile_items",
-        "num_joins", "join_rows", "part_rows", "table_at", "slots_at", "pages_at", "row_items_at", "tile_items_at",
-        "joins_at")] + [("seal", ctypes.c_uint64), ("device", ctypes.c_int64)]
+        "num_kv_heads", "head_dim", "all_new", "dtype", "row_tiles", "num_row_tiles", "num_row_groups",
+        "num_tile_items", "num_joins", "join_rows", "part_rows", "row_part_rows", "item_part_rows", "table_at",
+        "slots_at", "pages_at", "row_tiles_at", "row_starts_at", "tile_items_at", "joins_at")] + [("seal", ctypes.c_uint64), ("device", ctypes.c_int64)]
 
 
 class KvmCache(ctypes.Structure):

@@ -7,6 +7,7 @@
 // the block table).
 #include "kv_internal.h"
 #include "kvcache_rows.h"
+#include "kvcache_slow.h"
 #include "kvcache_tiles.h"
 
 #include <cmath>
@@ -127,49 +128,112 @@ __global__ __launch_bounds__(256) void kvm_read_kernel(const MoveArgs a)
 
 // ---- attention
 
+// A workgroup for few rows walks its share of the units of all (row tile, KV head) pairs: perhaps the end of
+// a pair, then whole ones, then the beginning of one.  The next piece's first loads are under way while a
+// piece's rows are joined and written.
 template <typename T, int SRC, int DP, int RT>
-__global__ __launch_bounds__(256) void kvm_rows_kernel(const AttnArgs a)
+__global__ __launch_bounds__(256, DP <= 64 ? 4 - RT : DP <= 128 ? 2 : 1) void kvm_rows_kernel(const AttnArgs a)
 {
-    __shared__ __attribute__((aligned(16))) char lds[RowShape<T, DP, RT>::kLds];
-    const uint32_t item_id = div_by(blockIdx.x, a.by_heads);
-    attend_rows<T, SRC, DP, RT>(a, a.items[item_id], blockIdx.x - item_id * a.heads, lds);
+    typedef Rows<T, SRC, DP, RT> R;
+    __shared__ __attribute__((aligned(16))) char lds[R::kLds];
+    R rows(a, lds);
+    KvStart at;
+    KvTile t;
+    auto first = [&]() {
+        at = uniform(a.starts + blockIdx.x);
+        t = uniform(a.tiles + at.tile);
+    };
+    auto piece = [&]() {
+        RowWork w;
+        const int n = min(at.units, t.units - at.unit);
+        w.q_start = t.q_start;
+        w.rows = t.rows;
+        w.first = t.first;
+        w.table_at = t.table_at;
+        w.row0 = t.row0;
+        w.head = at.head;
+        w.kv_begin = at.unit * (int)kUnit;
+        w.kv_end = min(t.kv_end, (at.unit + n) * (int)kUnit);
+        w.part_row = n == t.units ? -1 : (int64_t)(at.unit == 0 ? a.part_starts : 0) + (int64_t)blockIdx.x * a.part_pitch;
+        at.units -= n;
+        at.unit = 0;
+        if (++at.head == (int)a.heads) {
+            at.head = 0;
+            ++at.tile;
+            if (at.units > 0) t = uniform(a.tiles + at.tile);
+        }
+        return w;
+    };
+    first();
+    RowWork now = piece();
+    rows.begin(now);
+    for (;;) {
+        rows.run(now);
+        if (at.units == 0) break;
+        const RowWork next = piece();
+        rows.begin(next);
+        rows.finish(now);
+        now = next;
+    }
+    rows.finish(now);
+    // some piece met an infinity or a NaN that not all of its rows may see: all pieces once more, row by row
+    if (__builtin_expect(__syncthreads_or(rows.odd), 0)) {
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // the rows written above are to be written over
+        __syncthreads();
+        first();
+        while (at.units > 0) attend_slow<T, SRC, DP>(a, piece(), RT * 16);
+    }
 }
 
-// Partial rows into output rows: one row of one KV head for each LANES lanes.
+// Partial rows into output rows: LANES lanes a row.
 struct JoinArgs {
     const KvJoin *joins;
     const float *part_acc, *part_ml;
     char *out;
     uint64_t out_token, out_head;
-    uint32_t heads, group, head_dim, num_joins;
-    Divider by_heads, by_group;
+    uint32_t group, head_dim;
+    Divider by_group;
 };
 
+// The lanes of a row look at the pieces' maxima and sums side by side; then the pieces' rows are added up, a few
+// loads in flight at a time.
 template <typename T, int LANES>
 __global__ __launch_bounds__(256) void kvm_join_kernel(const JoinArgs a)
 {
-    const uint32_t join_id = div_by(blockIdx.x, a.by_heads), h = blockIdx.x - join_id * a.heads;
-    const KvJoin j = a.joins[join_id];
-    const int d = threadIdx.x % LANES * 8;
+    const KvJoin j = a.joins[blockIdx.x];
+    const int lane = threadIdx.x % LANES, d = lane * 8;
     const int r = blockIdx.y * (256 / LANES) + threadIdx.x / LANES;
-    if (r >= j.rows || d >= (int)a.head_dim) return;
-    float top = -INFINITY;
-    for (int p = 0; p < j.pieces; ++p)
-        top = fmaxf(top, a.part_ml[((uint64_t)(j.part_row + p * j.pitch + r) * a.heads + h) * 2]);
-    const float safe = top == -INFINITY ? 0.0f : top;
+    if (r >= j.rows) return;                       // a row's lanes leave together
+    auto part_row = [&](int p) { return (uint64_t)(uint32_t)(p == 0 ? j.part_row : j.next_row + (p - 1) * j.pitch) + r; };
+    float top = -INFINITY, sum = 0.0f;
+    for (int p = lane; p < j.pieces; p += LANES) {
+        const f32x2 ml = *(const f32x2 *)(a.part_ml + part_row(p) * 2);
+        const float m = fmaxf(top, ml[0]);
+        const float safe = m == -INFINITY ? 0.0f : m;
+        sum = sum * exp2_of(top - safe) + ml[1] * exp2_of(ml[0] - safe);
+        top = m;
+    }
+    float all = top;
+#pragma unroll
+    for (int x = 1; x < LANES; x <<= 1) all = fmaxf(all, __shfl_xor(all, x));
+    const float safe = all == -INFINITY ? 0.0f : all;
+    sum *= exp2_of(top - safe);
+#pragma unroll
+    for (int x = 1; x < LANES; x <<= 1) sum += __shfl_xor(sum, x);
+    if (d >= (int)a.head_dim) return;
     f32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-    float sum = 0.0f;
+#pragma unroll 4
     for (int p = 0; p < j.pieces; ++p) {
-        const uint64_t at = (uint64_t)(j.part_row + p * j.pitch + r) * a.heads + h;
-        const f32x2 ml = *(const f32x2 *)(a.part_ml + at * 2);
-        const float f = exp2_of(ml[0] - safe);
-        sum += f * ml[1];
-        x += f * *(const f32x4 *)(a.part_acc + at * a.head_dim + d);
-        y += f * *(const f32x4 *)(a.part_acc + at * a.head_dim + d + 4);
+        const uint64_t at = part_row(p);
+        const float f = exp2_of(a.part_ml[at * 2] - safe);
+        const f32x4 *from = (const f32x4 *)(a.part_acc + at * a.head_dim + d);
+        x += f * from[0];
+        y += f * from[1];
     }
     const uint32_t row = (uint32_t)(j.row0 + r), token = div_by(row, a.by_group), g = row - token * a.group;
     typedef typename Elem<T>::V4 V4;
-    V4 *o = (V4 *)(a.out + (uint64_t)(j.q_start + token) * a.out_token + (uint64_t)(h * a.group + g) * a.out_head + d * sizeof(T));
+    V4 *o = (V4 *)(a.out + (uint64_t)(j.q_start + token) * a.out_token + (uint64_t)((uint32_t)j.head * a.group + g) * a.out_head +
+                   d * sizeof(T));
     const float inverse = 1.0f / sum;
     o[0] = __builtin_convertvector(x * inverse, V4);
     o[1] = __builtin_convertvector(y * inverse, V4);
@@ -350,7 +414,7 @@ template <typename T, bool Q> int launch_read_q(const MoveArgs &a, uint64_t page
 
 template <typename T, int SRC, int DP> int launch_rows_d(const AttnArgs &a, const KvmStep *step, hipStream_t stream)
 {
-    const dim3 grid((uint32_t)(step->num_row_items * step->num_kv_heads));
+    const dim3 grid((uint32_t)step->num_row_groups);
     if constexpr (DP <= 128) {
         if (step->row_tiles == 2) kvm_rows_kernel<T, SRC, DP, 2><<<grid, 256, 0, stream>>>(a);
     }
@@ -372,10 +436,10 @@ template <int SRC> int launch_rows_t(const AttnArgs &a, const KvmStep *step, hip
     return launch_rows<float, SRC>(a, step, stream);
 }
 
-template <typename T> int launch_join(const JoinArgs &a, int64_t join_rows, hipStream_t stream)
+template <typename T> int launch_join(const JoinArgs &a, uint32_t num_joins, int64_t join_rows, hipStream_t stream)
 {
     const uint32_t lanes = a.head_dim <= 64 ? 8 : a.head_dim <= 128 ? 16 : 32, rows = 256 / lanes;
-    const dim3 grid(a.num_joins * a.heads, (uint32_t)((join_rows + rows - 1) / rows));
+    const dim3 grid(num_joins, (uint32_t)((join_rows + rows - 1) / rows));
     if (lanes == 8) kvm_join_kernel<T, 8><<<grid, 256, 0, stream>>>(a);
     else if (lanes == 16) kvm_join_kernel<T, 16><<<grid, 256, 0, stream>>>(a);
     else kvm_join_kernel<T, 32><<<grid, 256, 0, stream>>>(a);
@@ -397,8 +461,7 @@ int attend(const KvmStep *step, const int32_t *words, AttnArgs a, int format, co
                           (long long)(workspace ? workspace_bytes : 0), (long long)need);
         KV_TRY(check_memory(step, workspace, (uint64_t)need, workspace_bytes, "the workspace", &device));
     }
-    if ((uint64_t)((step->num_row_items + step->num_tile_items) * step->num_kv_heads) > kMaxGroups ||
-        (uint64_t)(step->num_joins * step->num_kv_heads) * 16 > kMaxGroups)
+    if ((uint64_t)(step->num_tile_items * step->num_kv_heads) > kMaxGroups || (uint64_t)step->num_joins * 16 > kMaxGroups)
         return refuse(KVM_EINVAL, "too many rows for one launch");
     const uint64_t size = (uint64_t)type_bytes(step->dtype);
     a.table = words + step->table_at;
@@ -419,15 +482,19 @@ int attend(const KvmStep *step, const int32_t *words, AttnArgs a, int format, co
     a.scale_log2 = fmaxf(fabsf(scale) * 1.44269504088896340736f, 1.2e-38f);
     a.q_sign = scale >= 0 ? 0u : size == 4 ? 0x80000000u : 0x80008000u;
     a.part_acc = (float *)workspace;
-    a.part_ml = a.part_acc + step->part_rows * step->num_kv_heads * step->head_dim;
+    a.part_ml = a.part_acc + step->part_rows * step->head_dim;
+    a.part_pitch = (uint32_t)(16 * step->row_tiles);
+    a.part_starts = (uint32_t)(step->num_row_groups * 16 * step->row_tiles);
+    a.part_items = (uint32_t)step->row_part_rows;
+    a.part_head = (uint32_t)step->item_part_rows;
     OnDevice on(device);
     KV_TRY(on.status);
-    if (step->num_tile_items > 0) {
-        a.items = (const KvItem *)(words + step->tile_items_at);
+    a.tiles = (const KvTile *)(words + step->row_tiles_at);
+    a.starts = (const KvStart *)(words + step->row_starts_at);
+    a.items = (const KvItem *)(words + step->tile_items_at);
+    if (step->num_tile_items > 0)
         KV_TRY(kvm_launch_tiles(a, (int)step->dtype, format, (uint32_t)(step->num_tile_items * step->num_kv_heads), stream));
-    }
-    if (step->num_row_items > 0) {
-        a.items = (const KvItem *)(words + step->row_items_at);
+    if (step->num_row_groups > 0) {
         if (format == kPacked) KV_TRY(launch_rows_t<kPacked>(a, step, stream));
         else if (format == kE4m3) KV_TRY(launch_rows_t<kE4m3>(a, step, stream));
         else KV_TRY(launch_rows_t<kPlain>(a, step, stream));
@@ -440,15 +507,12 @@ int attend(const KvmStep *step, const int32_t *words, AttnArgs a, int format, co
     j.out = a.out;
     j.out_token = a.out_token;
     j.out_head = a.out_head;
-    j.heads = a.heads;
     j.group = a.group;
     j.head_dim = a.head_dim;
-    j.num_joins = (uint32_t)step->num_joins;
-    j.by_heads = a.by_heads;
     j.by_group = a.by_group;
-    if (step->dtype == KVM_F16) return launch_join<_Float16>(j, step->join_rows, stream);
-    if (step->dtype == KVM_BF16) return launch_join<__bf16>(j, step->join_rows, stream);
-    return launch_join<float>(j, step->join_rows, stream);
+    if (step->dtype == KVM_F16) return launch_join<_Float16>(j, (uint32_t)step->num_joins, step->join_rows, stream);
+    if (step->dtype == KVM_BF16) return launch_join<__bf16>(j, (uint32_t)step->num_joins, step->join_rows, stream);
+    return launch_join<float>(j, (uint32_t)step->num_joins, step->join_rows, stream);
 }
 
 }  // namespace

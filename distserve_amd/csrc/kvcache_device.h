@@ -116,7 +116,9 @@ __device__ inline uint32_t div_by(uint32_t n, Divider d) { return (uint32_t)(((u
 // ---- the attention kernels' arguments
 
 struct AttnArgs {
-    const KvItem *items;
+    const KvTile *tiles;                      // few rows
+    const KvStart *starts;
+    const KvItem *items;                      // many rows
     const int32_t *table;
     const char *q;
     char *out;
@@ -128,10 +130,31 @@ struct AttnArgs {
     Divider by_block, by_heads, by_group;
     float scale_log2;                         // |scale| * log2(e): the softmax is taken in powers of two
     uint32_t q_sign;                          // sign bits of q to turn over (a negative scale)
-    float *part_acc, *part_ml;                // partial rows: [row][kv head][head_dim], and {maximum, sum}
+    float *part_acc, *part_ml;                // partial rows: [row][head_dim], and {maximum, sum}
+    uint32_t part_starts, part_pitch;         // few rows: workgroup w's partial rows for a pair it starts (begins anew) with are at
+                                              // w * part_pitch, for one it leaves unfinished at part_starts + w * part_pitch
+    uint32_t part_items, part_head;           // many rows: KV head h's partial rows start at part_items + h * part_head
+};
+
+// Rows row0 .. of a sequence for one KV head over keys [kv_begin, kv_end).
+struct RowWork {
+    int q_start, rows, first, table_at, row0;   // as in KvTile
+    int head;
+    int kv_begin, kv_end;
+    int64_t part_row;                           // partial rows start here; -1: these are all of the rows' keys
 };
 
 enum { kPlain = 0, kE4m3 = 1, kPacked = 2 };
+
+// A structure of words that is the same for the whole wave, in scalar registers.
+template <typename S> __device__ inline S uniform(const S *p)
+{
+    union { S s; int w[sizeof(S) / 4]; } u;
+    u.s = *p;
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(S) / 4; ++i) u.w[i] = __builtin_amdgcn_readfirstlane(u.w[i]);
+    return u.s;
+}
 
 template <typename V> __device__ inline V as(u32x4 w)
 {

@@ -4,11 +4,11 @@
 //   table   the block tables, one sequence after the other
 //   slots   for each new token, its cache slot (block * block_size + offset)
 //   pages   for each table entry, {first row of the read-back output, tokens in the block}
-//   row items, tile items   the attention's work lists (KvItem), longest first
+//   row tiles, row starts   the attention's work for few rows (KvTile, KvStart)
+//   tile items              ... and for many (KvItem)
 //   joins   which partial rows make up which output rows (KvJoin)
 // Lengths, block ids and the write set are checked while it is built, so no kernel can be
-// sent outside a pool by a plan, and the work list is balanced over the whole batch: long
-// sequences are cut into pieces of the length that spreads the step's keys over the chip.
+// sent outside a pool by a plan, and the work is balanced over the whole batch.
 #include "kvcache_plan.h"
 #include "kv_internal.h"
 
@@ -35,6 +35,9 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Sequences' sums stay in int32 (words of the plan), with room for a tile's overhang.
 constexpr int64_t kMaxTokens = (1ll << 31) - 4096;
 
+// Workgroups of the kernel for few rows that run at the same time: what its registers allow for a head_dim.
+int64_t most_groups(int64_t head_dim) { return kCus * (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1); }
+
 }  // namespace
 
 uint64_t kvm_step_seal(const KvmStep &s)
@@ -57,8 +60,9 @@ int64_t kvm_plan_words(int64_t num_seqs, int64_t num_tokens, int64_t num_pages, 
     if (num_seqs < 0 || num_tokens < 0 || num_pages < 0 || num_heads < 1 || num_kv_heads < 1) return KVM_EINVAL;
     const int64_t group = std::max<int64_t>(1, num_heads / num_kv_heads);
     const int64_t tiles = num_seqs + num_tokens * group / 16;            // one at least for each sequence
-    const int64_t items = 2 * tiles + 2 * kTargetWorkgroups + 64;            // a cut adds one piece for each piece length
-    return 64 + num_pages * 3 + num_tokens + items * kItemWords + tiles * kJoinWords;
+    const int64_t big = num_seqs + num_tokens * group / kTileRows;
+    return 64 + num_pages * 3 + num_tokens + tiles * kTileWords + most_groups(16) * (kStartWords + kJoinWords) +
+           (2 * big + kTileTarget) * kItemWords + big * num_kv_heads * kJoinWords;
 }
 
 int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t num_seqs, const int64_t *table,
@@ -126,8 +130,8 @@ int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t
     out.table_at = 0;
     out.pages_at = (pages + 1) / 2 * 2;
     out.slots_at = out.pages_at + 2 * pages;
-    out.row_items_at = (out.slots_at + slots + 3) / 4 * 4;
-    if (out.row_items_at > capacity)
+    out.row_tiles_at = (out.slots_at + slots + 3) / 4 * 4;
+    if (out.row_tiles_at > capacity)
         return refuse(KVM_EINVAL, "kvm_plan_step: %lld words are too few, kvm_plan_words says how many", (long long)capacity);
 
     if (cached) {
@@ -179,69 +183,120 @@ int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t
     // two 16-row tiles share the keys that a wave loads, where the registers hold their accumulators
     out.row_tiles = most_rows > 16 && head_dim <= 128 ? 2 : 1;
 
-    int64_t part = 0, join_rows = 0;
-    std::vector<KvItem> items[2];   // few rows, many rows
+    // few rows: the keys of all (row tile, KV head) pairs in a row, dealt out evenly in units
+    std::vector<KvTile> tiles;
+    std::vector<KvStart> starts;
     std::vector<KvJoin> joins;
-    for (int many = 0; many < 2; ++many) {
-        const int64_t tile_rows = many ? kTileRows : 16 * out.row_tiles;
-        const int64_t step_keys = many ? kTileStep : kPieceStep;
-        int64_t keys = 0;
-        for (int64_t s = 0; s < num_seqs; ++s)
-            for (int64_t r = 0; in_tiles(s) == (many != 0) && r < new_tokens[s] * group; r += tile_rows)
-                keys += first_token[s] + (std::min(r + tile_rows, new_tokens[s] * group) - 1) / group + 1;
-        const int64_t piece = std::max<int64_t>(ceil_div(ceil_div(keys * num_kv_heads, kTargetWorkgroups), step_keys) * step_keys,
-                                                many ? kMinTilePiece : kMinPiece);
-        int64_t q_start = 0, table_at = 0;
-        for (int64_t s = 0; s < num_seqs; ++s) {
-            const int64_t rows = new_tokens[s] * group;
-            for (int64_t r = 0; in_tiles(s) == (many != 0) && r < rows; r += tile_rows) {
-                const int64_t here = std::min(tile_rows, rows - r);
-                const int64_t end = first_token[s] + (r + here - 1) / group + 1;
-                const int64_t cuts = std::max<int64_t>(1, end / piece + (end % piece > piece / 2 ? 1 : 0));
-                const int64_t len = ceil_div(ceil_div(end, cuts), step_keys) * step_keys;
-                const int64_t pieces = ceil_div(end, len);
-                KvItem it;
-                it.q_start = (int32_t)q_start;
-                it.rows = (int32_t)rows;
-                it.first = (int32_t)first_token[s];
-                it.table_at = (int32_t)table_at;
-                it.row0 = (int32_t)r;
-                for (int64_t p = 0; p < pieces; ++p) {
-                    it.kv_begin = (int32_t)(p * len);
-                    it.kv_end = (int32_t)std::min(end, (p + 1) * len);
-                    it.part_row = pieces > 1 ? (int32_t)(part + p * here) : -1;
-                    items[many].push_back(it);
-                }
-                if (pieces > 1) {
-                    joins.push_back(KvJoin{(int32_t)q_start, (int32_t)r, (int32_t)here, (int32_t)part, (int32_t)here,
-                                           (int32_t)pieces, 0, 0});
-                    part += pieces * here;
+    int64_t units = 0, join_rows = 0, q_start = 0, table_at = 0;
+    const int64_t tile_rows = 16 * out.row_tiles;
+    for (int64_t s = 0; s < num_seqs; ++s) {
+        const int64_t rows = new_tokens[s] * group;
+        for (int64_t r = 0; !in_tiles(s) && r < rows; r += tile_rows) {
+            const int64_t end = first_token[s] + (std::min(r + tile_rows, rows) - 1) / group + 1;
+            tiles.push_back(KvTile{(int32_t)q_start, (int32_t)rows, (int32_t)first_token[s], (int32_t)table_at, (int32_t)r,
+                                   (int32_t)end, (int32_t)ceil_div(end, kUnit), 0});
+            units += ceil_div(end, kUnit) * num_kv_heads;
+        }
+        q_start += new_tokens[s];
+        if (cached) table_at += table_len[s];
+    }
+    const int64_t groups = std::min(most_groups(head_dim), ceil_div(units, kMinUnits));
+    {
+        size_t tile = 0;
+        int64_t head = 0, unit = 0, open = -1;   // open: the group that began the pair at hand and left it unfinished
+        for (int64_t w = 0; w < groups; ++w) {
+            int64_t left = units / groups + (w < units % groups ? 1 : 0);
+            starts.push_back(KvStart{(int32_t)tile, (int32_t)head, (int32_t)unit, (int32_t)left});
+            while (left > 0) {
+                const KvTile &t = tiles[tile];
+                const int64_t n = std::min<int64_t>(left, t.units - unit);
+                if (unit == 0 && n < t.units) open = w;
+                left -= n;
+                unit += n;
+                if (unit < t.units) break;
+                if (open >= 0) {
+                    const int64_t here = std::min<int64_t>(tile_rows, t.rows - t.row0);
+                    joins.push_back(KvJoin{t.q_start, t.row0, (int32_t)here, (int32_t)head, (int32_t)((groups + open) * tile_rows),
+                                           (int32_t)((open + 1) * tile_rows), (int32_t)tile_rows, (int32_t)(w - open + 1)});
                     join_rows = std::max(join_rows, here);
-                    if (part > kMaxTokens) return refuse(KVM_EINVAL, "a step of more than 2^31 partial rows is not supported");
+                    open = -1;
+                }
+                unit = 0;
+                if (++head == num_kv_heads) {
+                    head = 0;
+                    ++tile;
                 }
             }
-            q_start += new_tokens[s];
-            if (cached) table_at += table_len[s];
         }
-        // the longest pieces first, so that the last workgroups to start are short
-        std::stable_sort(items[many].begin(), items[many].end(), [](const KvItem &a, const KvItem &b) {
-            return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin;
-        });
     }
-    out.num_row_items = (int64_t)items[0].size();
-    out.num_tile_items = (int64_t)items[1].size();
+    out.row_part_rows = joins.empty() ? 0 : 2 * groups * tile_rows;
+
+    // many rows: 128-row tiles, their keys cut where that spreads the step over the chip
+    std::vector<KvItem> items;
+    int64_t keys = 0, part = 0;
+    for (int64_t s = 0; s < num_seqs; ++s)
+        for (int64_t r = 0; in_tiles(s) && r < new_tokens[s] * group; r += kTileRows)
+            keys += first_token[s] + (std::min(r + kTileRows, new_tokens[s] * group) - 1) / group + 1;
+    const int64_t piece = std::max(ceil_div(ceil_div(keys * num_kv_heads, kTileTarget), kTileStep) * kTileStep, kMinTilePiece);
+    std::vector<KvJoin> cut;
+    q_start = table_at = 0;
+    for (int64_t s = 0; s < num_seqs; ++s) {
+        const int64_t rows = new_tokens[s] * group;
+        for (int64_t r = 0; in_tiles(s) && r < rows; r += kTileRows) {
+            const int64_t here = std::min(kTileRows, rows - r);
+            const int64_t end = first_token[s] + (r + here - 1) / group + 1;
+            const int64_t cuts = std::max<int64_t>(1, end / piece + (end % piece > piece / 2 ? 1 : 0));
+            const int64_t len = ceil_div(ceil_div(end, cuts), kTileStep) * kTileStep;
+            const int64_t pieces = ceil_div(end, len);
+            for (int64_t p = 0; p < pieces; ++p)
+                items.push_back(KvItem{(int32_t)q_start, (int32_t)rows, (int32_t)first_token[s], (int32_t)table_at, (int32_t)r,
+                                       (int32_t)(p * len), (int32_t)std::min(end, (p + 1) * len),
+                                       pieces > 1 ? (int32_t)(part + p * here) : -1});
+            if (pieces > 1) {
+                cut.push_back(KvJoin{(int32_t)q_start, (int32_t)r, (int32_t)here, 0, (int32_t)part, (int32_t)(part + here),
+                                     (int32_t)here, (int32_t)pieces});
+                part += pieces * here;
+                join_rows = std::max(join_rows, here);
+            }
+            if (part * num_kv_heads > kMaxTokens) return refuse(KVM_EINVAL, "a step of more than 2^31 partial rows is not supported");
+        }
+        q_start += new_tokens[s];
+        if (cached) table_at += table_len[s];
+    }
+    // the longest pieces first, so that the last workgroups to start are short
+    std::stable_sort(items.begin(), items.end(),
+                     [](const KvItem &a, const KvItem &b) { return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin; });
+    out.item_part_rows = part;
+    out.part_rows = out.row_part_rows + part * num_kv_heads;
+    if (out.part_rows > kMaxTokens) return refuse(KVM_EINVAL, "a step of more than 2^31 partial rows is not supported");
+    for (const KvJoin &j : cut)
+        for (int64_t h = 0; h < num_kv_heads; ++h) {
+            KvJoin of_head = j;
+            of_head.head = (int32_t)h;
+            of_head.part_row += (int32_t)(out.row_part_rows + h * part);
+            of_head.next_row += (int32_t)(out.row_part_rows + h * part);
+            joins.push_back(of_head);
+        }
+
+    out.num_row_tiles = (int64_t)tiles.size();
+    out.num_row_groups = groups;
+    out.num_tile_items = (int64_t)items.size();
     out.num_joins = (int64_t)joins.size();
     out.join_rows = join_rows;
-    out.part_rows = part;
-    out.tile_items_at = out.row_items_at + out.num_row_items * kItemWords;
-    out.joins_at = out.tile_items_at + out.num_tile_items * kItemWords;
-    out.words = out.joins_at + out.num_joins * kJoinWords;
+    int64_t at = out.row_tiles_at;
+    auto section = [&](const void *from, size_t bytes) {
+        const int64_t here = at;
+        at += (int64_t)bytes / 4;
+        if (at <= capacity && bytes > 0) memcpy(words + here, from, bytes);
+        return here;
+    };
+    section(tiles.data(), tiles.size() * sizeof(KvTile));
+    out.row_starts_at = section(starts.data(), starts.size() * sizeof(KvStart));
+    out.tile_items_at = section(items.data(), items.size() * sizeof(KvItem));
+    out.joins_at = section(joins.data(), joins.size() * sizeof(KvJoin));
+    out.words = at;
     if (out.words > capacity)
         return refuse(KVM_EINVAL, "kvm_plan_step: %lld words are too few, kvm_plan_words says how many", (long long)capacity);
-    for (int many = 0; many < 2; ++many)
-        if (!items[many].empty())
-            memcpy(words + (many ? out.tile_items_at : out.row_items_at), items[many].data(), items[many].size() * sizeof(KvItem));
-    if (!joins.empty()) memcpy(words + out.joins_at, joins.data(), joins.size() * sizeof(KvJoin));
     out.seal = kvm_step_seal(out);
     out.device = -1;
     *step = out;
@@ -251,7 +306,7 @@ int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t
 int64_t kvm_attention_workspace(const KvmStep *step)
 {
     if (!step || step->seal != kvm_step_seal(*step)) return refuse(KVM_EINVAL, "the step is not one kvm_plan_step made");
-    return step->part_rows * step->num_kv_heads * (step->head_dim + 2) * (int64_t)sizeof(float);
+    return step->part_rows * (step->head_dim + 2) * (int64_t)sizeof(float);
 }
 
 }  // extern "C"

@@ -6,32 +6,48 @@
 
 #include <cstddef>
 
-// A piece of attention work for one KV head: rows row0 .. of a sequence over keys [kv_begin, kv_end).
-struct KvItem {
+// A row tile of a sequence, for the kernel for few rows: the same for every KV head.
+struct KvTile {
     int32_t q_start;    // first token row of the sequence in q and out
     int32_t rows;       // query rows of the sequence for one KV head: new tokens x heads of the group
     int32_t first;      // tokens before the step
     int32_t table_at;   // where the sequence's block table starts
     int32_t row0;
+    int32_t kv_end;     // keys that the tile's last row may see
+    int32_t units, pad; // of kUnit keys
+};
+
+// Where a workgroup of the kernel for few rows starts: the units of all (tile, KV head) pairs in a row are
+// dealt out evenly, so that every workgroup has the same amount to read.
+struct KvStart {
+    int32_t tile, head, unit, units;
+};
+
+// A piece of attention work for the kernel for many rows, for every KV head: rows row0 .. over keys [kv_begin, kv_end).
+struct KvItem {
+    int32_t q_start, rows, first, table_at, row0;   // as above
     int32_t kv_begin, kv_end;
-    int32_t part_row;   // first partial row of this piece, -1 when the piece is the whole row
+    int32_t part_row;   // first partial row of this piece for KV head 0, -1 when the piece is the whole row
 };
 
-// Rows whose keys were cut into pieces: piece p's partial rows start at part_row + p * pitch.
+// Rows of one KV head whose keys were cut into pieces: partial rows start at part_row, then at next_row + i * pitch.
 struct KvJoin {
-    int32_t q_start, row0, rows, part_row, pitch, pieces, pad0, pad1;
+    int32_t q_start, row0, rows, head, part_row, next_row, pitch, pieces;
 };
 
+constexpr int64_t kTileWords = sizeof(KvTile) / 4;
+constexpr int64_t kStartWords = sizeof(KvStart) / 4;
 constexpr int64_t kItemWords = sizeof(KvItem) / 4;
 constexpr int64_t kJoinWords = sizeof(KvJoin) / 4;
 
-constexpr int64_t kTargetWorkgroups = 1024;   // four for each of the 256 CUs
-constexpr int64_t kPieceStep = 128;           // keys the four waves of a workgroup take in one turn
-constexpr int64_t kMinPiece = 256;
+constexpr int64_t kUnit = 128;                // keys the four waves of a workgroup for few rows take in one turn
+constexpr int64_t kCus = 256;
+constexpr int64_t kMinUnits = 2;              // a workgroup for few rows takes at least, so that the joins stay few
 constexpr int64_t kFewRows = 32;              // up to here a sequence's rows go to the kernel for few rows
 constexpr int64_t kTileRows = 128;            // of a workgroup of the kernel for many rows
 constexpr int64_t kTileStep = 64;             // keys of its tiles
-constexpr int64_t kMinTilePiece = 512;
+constexpr int64_t kTileTarget = 1024;         // workgroups it is cut into at least, if the pieces stay above
+constexpr int64_t kMinTilePiece = 512;        // this many keys
 
 uint64_t kvm_step_seal(const KvmStep &s);
 

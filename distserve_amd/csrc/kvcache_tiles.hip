@@ -10,7 +10,7 @@
 // (quantised pools).  A row's 16-byte chunks are swapped around by the row's number, so that the 16
 // rows of an operand read, and the four rows of a transposing read, fall into different banks.
 #include "kv_internal.h"
-#include "kvcache_rows.h"
+#include "kvcache_slow.h"
 #include "kvcache_tiles.h"
 
 #include <cstdio>
@@ -44,7 +44,6 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
     static constexpr int kDt = DP / 32;                 // 32-wide tiles of head_dim in the output
     static constexpr int kRowsPerLoad = 1024 / kRow;    // rows of a wave's 16-byte-a-lane load
     static constexpr int kLoads = 16 / kRowsPerLoad;    // a wave brings 16 of the 64 rows
-    static_assert(RowShape<T, DP, 1>::kLds <= kLds, "the rows' code runs in the tiles' LDS");
     static constexpr int kCoded = DP / 64;              // quantised: 16-code loads of a lane for a row
 
     static __device__ int swizzle_k(int row) { return DP == 64 ? (row >> 1) & 7 : row & 15; }
@@ -285,10 +284,13 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
     }
 
     __device__ TileKernel(const AttnArgs &args, char *shared, uint32_t item_id, uint32_t head)
-        : a(args), it(args.items[item_id]), h((int)head), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
+        : a(args), it(uniform(args.items + item_id)), h((int)head), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
           lane(threadIdx.x & 63), col(threadIdx.x & 31), half((threadIdx.x & 63) >> 5), lds(shared)
     {
     }
+
+    // the item's first partial row
+    __device__ int64_t part_at() const { return (int64_t)a.part_items + (int64_t)h * a.part_head + it.part_row; }
 
     __device__ void run()
     {
@@ -312,13 +314,10 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
             }
         }
         if (!pass(first_row)) {
-            __builtin_amdgcn_s_waitcnt(0x0f70);   // loads into LDS may still be on their way
-            const int end = min(it.row0 + QT * 128, it.rows);
-            for (KvItem few = it; few.row0 < end; few.row0 += 16) {
-                __syncthreads();
-                few.part_row = it.part_row < 0 ? -1 : it.part_row + (few.row0 - it.row0);
-                attend_rows<T, SRC, DP, 1>(a, few, (uint32_t)h, lds);
-            }
+            const RowWork all = {it.q_start, it.rows, it.first, it.table_at, it.row0, h, it.kv_begin, it.kv_end,
+                                 it.part_row < 0 ? -1 : part_at()};
+            attend_slow<T, SRC, DP>(a, all, QT * 128);
+            __builtin_amdgcn_s_waitcnt(0x0f70);   // the next tile may still be on its way into LDS
             return;
         }
 #pragma unroll
@@ -327,7 +326,7 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
             const float sum = l[qt] + __shfl_xor(l[qt], 32);
             if (r >= it.rows) continue;
             if (it.part_row >= 0) {
-                const uint64_t at = (uint64_t)(it.part_row + (r - it.row0)) * a.heads + h;
+                const uint64_t at = (uint64_t)part_at() + (r - it.row0);
 #pragma unroll
                 for (int dt = 0; dt < kDt; ++dt)
 #pragma unroll

@@ -293,10 +293,12 @@ typedef struct KvmStep {
     int64_t all_new;        /* 1 when no sequence has tokens before this step's */
     int64_t dtype;          /* KVM_F16, KVM_BF16 or KVM_F32 */
     int64_t row_tiles;      /* 16-row tiles of a workgroup of the kernel for few rows */
-    int64_t num_row_items, num_tile_items;   /* work for the kernel for few rows, for the one for many */
+    int64_t num_row_tiles, num_row_groups;   /* its row tiles, its workgroups */
+    int64_t num_tile_items;                  /* work items of the kernel for many rows */
     int64_t num_joins, join_rows;
-    int64_t part_rows;      /* partial rows for each KV head */
-    int64_t table_at, slots_at, pages_at, row_items_at, tile_items_at, joins_at;   /* sections, in words */
+    int64_t part_rows;      /* partial rows, both kernels' */
+    int64_t row_part_rows, item_part_rows;   /* the first kernel's, and the second's for each KV head */
+    int64_t table_at, slots_at, pages_at, row_tiles_at, row_starts_at, tile_items_at, joins_at;   /* sections, in words */
     uint64_t seal;          /* guards against a plan that was not made by kvm_plan_step */
     /* Set by the caller, -1 after kvm_plan_step: the device that the words were copied to, if the caller
      * vouches that every pointer of its calls with this step lies on that device and for the extents it

@@ -10,9 +10,41 @@ import cache_reference as ref
 from distserve_amd import cabi
 
 
-def items_of(step, words, many):
-    at, n = (step.tile_items_at, step.num_tile_items) if many else (step.row_items_at, step.num_row_items)
-    return [tuple(words[at + 8 * i:at + 8 * i + 8]) for i in range(n)]
+def section(words, at, n, width):
+    return [tuple(words[at + width * i:at + width * (i + 1)]) for i in range(n)]
+
+
+def pieces_of(step, words, heads):
+    """What the kernels make of a plan: {(q_start, row0, head): [(kv_begin, kv_end, part_row)]} of the kernel
+    for few rows and of the one for many, walked as the kernels walk it."""
+    few, many = {}, {}
+    tiles = section(words, step.row_tiles_at, step.num_row_tiles, 8)
+    height = 16 * step.row_tiles
+    at = (0, 0, 0)
+    for group, (tile, head, unit, units) in enumerate(section(words, step.row_starts_at, step.num_row_groups, 4)):
+        assert (tile, head, unit) == at and units > 0          # each group goes on where the one before stopped
+        while units:
+            q_start, rows, first, table_at, row0, kv_end, total, _ = tiles[tile]
+            n = min(units, total - unit)
+            part = -1 if n == total else (step.num_row_groups * height if unit == 0 else 0) + group * height
+            few.setdefault((q_start, row0, head), []).append((unit * 128, min(kv_end, (unit + n) * 128), part))
+            units -= n
+            unit += n
+            if unit == total:
+                unit, head = 0, head + 1
+                if head == heads:
+                    head, tile = 0, tile + 1
+        at = (tile, head, unit)
+    assert at == (step.num_row_tiles, 0, 0)                    # and nothing is left over
+    lengths = []
+    for q_start, rows, first, table_at, row0, kv0, kv1, part in section(words, step.tile_items_at, step.num_tile_items, 8):
+        assert kv0 % 64 == 0
+        lengths.append(kv1 - kv0)
+        for head in range(heads):
+            at_head = -1 if part < 0 else step.row_part_rows + head * step.item_part_rows + part
+            many.setdefault((q_start, row0, head), []).append((kv0, kv1, at_head))
+    assert lengths == sorted(lengths, reverse=True)
+    return few, many
 
 
 def plan(first, new, table, num_blocks=64, block_size=16, heads=8, kv_heads=2, head_dim=64, dtype=cabi.KVM_F16):
@@ -53,42 +85,38 @@ def test_the_pieces_of_a_plan_cover_every_row_and_key_once(heads, kv_heads, head
         for b, p in zip(new, pages):
             starts.append(starts[-1] + b)
             table_at.append(table_at[-1] + p)
-        rows = {}
         tile_of = [128 if dtype != cabi.KVM_F32 and m * group > 32 else 16 * step.row_tiles for m in new]
-        for many in (0, 1):
-            lengths = []
-            for q_start, total, begin, table_start, row0, kv0, kv1, part in items_of(step, words, many):
-                owners = [s for s in range(n) if starts[s] == q_start and new[s] > 0]
-                assert len(owners) == 1
-                s = owners[0]
+        # the tiles' and items' own fields
+        for at, count in ((step.row_tiles_at, step.num_row_tiles), (step.tile_items_at, step.num_tile_items)):
+            for q_start, total, begin, table_start, row0, *_ in section(words, at, count, 8):
+                s = next(s for s in range(n) if starts[s] == q_start and new[s] > 0)
                 assert total == new[s] * group and begin == first[s] and table_start == table_at[s]
-                assert (tile_of[s] == 128) == bool(many)
-                assert 0 <= kv0 < kv1 <= first[s] + new[s] and row0 % tile_of[s] == 0
-                assert kv0 % (64 if many else 128) == 0
-                rows.setdefault((s, row0), []).append((kv0, kv1, part))
-                lengths.append(kv1 - kv0)
-            assert lengths == sorted(lengths, reverse=True)
-        joins = {}
-        for i in range(step.num_joins):
-            q_start, row0, here, part, pitch, pieces, _, _ = words[step.joins_at + 8 * i:step.joins_at + 8 * i + 8]
-            joins[q_start, row0] = (here, part, pitch, pieces)
+                assert (tile_of[s] == 128) == (at == step.tile_items_at) and row0 % tile_of[s] == 0
+        few, many = pieces_of(step, words, kv_heads)
+        joins = {(j[0], j[1], j[3]): j for j in section(words, step.joins_at, step.num_joins, 8)}
+        assert len(joins) == step.num_joins
         used = []
         for s in range(n):
             for row0 in range(0, new[s] * group, tile_of[s]):
-                pieces = sorted(rows.pop((s, row0)))
                 here = min(tile_of[s], new[s] * group - row0)
-                assert pieces[0][0] == 0 and pieces[-1][1] == first[s] + (row0 + here - 1) // group + 1
-                assert all(a[1] == b[0] for a, b in zip(pieces, pieces[1:]))
-                if len(pieces) == 1:
-                    assert pieces[0][2] == -1 and (starts[s], row0) not in joins
-                else:
-                    rows_here, part, pitch, count = joins.pop((starts[s], row0))
-                    assert rows_here == here == pitch and count == len(pieces) and here <= step.join_rows
-                    assert [p[2] for p in pieces] == [part + i * pitch for i in range(count)]
-                    used += [r for p in pieces for r in range(p[2], p[2] + here)]
-        assert not rows and not joins
-        assert sorted(used) == list(range(step.part_rows))
-        assert cabi.attention_workspace(step) == step.part_rows * kv_heads * (head_dim + 2) * 4
+                for head in range(kv_heads):
+                    key = (starts[s], row0, head)
+                    pieces = (many if tile_of[s] == 128 else few).pop(key)
+                    assert pieces[0][0] == 0 and pieces[-1][1] == first[s] + (row0 + here - 1) // group + 1
+                    assert all(a[1] == b[0] and a[0] < a[1] for a, b in zip(pieces, pieces[1:]))
+                    if len(pieces) == 1:
+                        assert pieces[0][2] == -1 and key not in joins
+                    else:
+                        _, _, rows_here, _, part, after, pitch, count = joins.pop(key)
+                        assert rows_here == here <= step.join_rows and count == len(pieces)
+                        assert [p[2] for p in pieces] == [part] + [after + i * pitch for i in range(count - 1)]
+                        used += [r for p in pieces for r in range(p[2], p[2] + here)]
+        assert not few and not many and not joins
+        assert len(set(used)) == len(used) and all(0 <= r < step.part_rows for r in used)
+        assert cabi.attention_workspace(step) == step.part_rows * (head_dim + 2) * 4
+        # every group of the kernel for few rows has the same amount to read, give or take a unit
+        shares = [g[3] for g in section(words, step.row_starts_at, step.num_row_groups, 4)]
+        assert not shares or max(shares) - min(shares) <= 1
 
 
 def test_plans_refuse_what_a_kernel_could_trip_over():
@@ -121,7 +149,7 @@ def test_plans_refuse_what_a_kernel_could_trip_over():
     assert step.num_blocks == 0 and step.num_tokens == 7
     # an empty step is a plan like any other
     step, _ = plan([], [], [])
-    assert step.num_tokens == 0 and step.num_row_items == 0
+    assert step.num_tokens == 0 and step.num_row_groups == 0 and step.num_tile_items == 0
     # too little room is refused, not overrun
     words, first, new = (ctypes.c_int32 * 64)(), (ctypes.c_int64 * 1)(0), (ctypes.c_int64 * 1)(40)
     table, lens, out = (ctypes.c_int64 * 3)(0, 1, 2), (ctypes.c_int64 * 1)(3), cabi.KvmStep()
