@@ -63,7 +63,7 @@ class KvmStep(ctypes.Structure):
 
     _fields_ = [(name, ctypes.c_int64) for name in (
         "words", "num_seqs", "num_tokens", "num_kv_tokens", "num_pages", "num_blocks", "block_size", "num_heads",
-        "num_kv_heads", "head_dim", "all_new", "dtype", "row_tiles", "num_row_tiles", "num_row_groups",
+        "num_kv_heads", "head_dim", "all_new", "dtype", "format", "row_tiles", "num_row_tiles", "num_row_groups",
         "num_tile_items", "num_joins", "join_rows", "part_rows", "row_part_rows", "item_part_rows", "table_at",
         "slots_at", "pages_at", "row_tiles_at", "row_starts_at", "tile_items_at", "joins_at")] + [("seal", ctypes.c_uint64), ("device", ctypes.c_int64)]
 
@@ -120,7 +120,7 @@ def _load(path: str) -> ctypes.CDLL:
     step, cache, rows = ctypes.POINTER(KvmStep), ctypes.POINTER(KvmCache), ctypes.POINTER(KvmRows)
     lib.kvm_plan_words.argtypes = [i64] * 5
     lib.kvm_plan_words.restype = i64
-    lib.kvm_plan_step.argtypes = [ip, ip, i64, ip, ip, i64, i64, i64, i64, i64, i32, i32p, i64, step]
+    lib.kvm_plan_step.argtypes = [ip, ip, i64, ip, ip, i64, i64, i64, i64, i64, i32, i32, i32p, i64, step]
     lib.kvm_write_kv.argtypes = [step, vp, cache, rows, rows, vp]
     lib.kvm_read_kv.argtypes = [step, vp, cache, rows, rows, vp]
     lib.kvm_attention_workspace.argtypes = [step]
@@ -251,7 +251,8 @@ class Binding:
     # ---- cache operators
 
     def plan_step(self, first_token: Sequence[int], new_tokens: Sequence[int], block_table: Sequence[Sequence[int]],
-                  num_blocks: int, block_size: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: int):
+                  num_blocks: int, block_size: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype: int,
+                  format: int = KVM_CACHE_PLAIN):
         """(KvmStep, the plan's words as a ctypes array): the words go to device memory as they are.
         ``num_blocks == 0``: a plan without a cache, ``block_table`` is ignored."""
         n = len(first_token)
@@ -263,8 +264,8 @@ class Binding:
         words = (ctypes.c_int32 * max(room, 64))()
         step = KvmStep()
         self._check(self.lib.kvm_plan_step(_arr(first_token), _arr(new_tokens), n, _arr(flat), _arr([len(t) for t in tables]),
-                                           num_blocks, block_size, num_heads, num_kv_heads, head_dim, dtype, words,
-                                           len(words), ctypes.byref(step)))
+                                           num_blocks, block_size, num_heads, num_kv_heads, head_dim, dtype, format,
+                                           words, len(words), ctypes.byref(step)))
         return step, words
 
     def write_kv(self, step: KvmStep, words: int, cache: KvmCache, k: KvmRows, v: KvmRows, stream: int = 0) -> None:

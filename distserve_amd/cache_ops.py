@@ -69,7 +69,7 @@ def plan_step(k_cache: torch.Tensor, input_lens: Sequence[int], first_token_inde
         raise RuntimeError("plan_step: the pool has no blocks")
     return StepPlan(list(first_token_indexes), list(input_lens), list(chain.from_iterable(block_table)),
                     [len(t) for t in block_table], num_blocks, block_size, num_heads, num_kv_heads,
-                    width - 1 if coded else width, _type_number(dtype), k_cache.device.index)
+                    width - 1 if coded else width, _type_number(dtype), coded, k_cache.device.index)
 
 
 def plan_prompt(input_lens: Sequence[int], num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype,
@@ -80,7 +80,7 @@ def plan_prompt(input_lens: Sequence[int], num_heads: int, num_kv_heads: int, he
         raise RuntimeError("plan_prompt: the operators run on the GPU")
     index = torch.cuda.current_device() if device.index is None else device.index
     lens = list(input_lens)
-    return StepPlan([0] * len(lens), lens, [], [], 0, 0, num_heads, num_kv_heads, head_dim, _type_number(dtype), index)
+    return StepPlan([0] * len(lens), lens, [], [], 0, 0, num_heads, num_kv_heads, head_dim, _type_number(dtype), False, index)
 
 
 def write_kv(plan: StepPlan, layer: int, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,

@@ -129,19 +129,20 @@ __global__ __launch_bounds__(256) void kvm_read_kernel(const MoveArgs a)
 // ---- attention
 
 // A workgroup for few rows walks its share of the units of all (row tile, KV head) pairs: perhaps the end of
-// a pair, then whole ones, then the beginning of one.  The next piece's first loads are under way while a
-// piece's rows are joined and written.
+// a pair, then whole ones, then the beginning of one.  The next piece's first K is under way while a piece's
+// rows are joined and written.
 template <typename T, int SRC, int DP, int RT>
-__global__ __launch_bounds__(256, DP <= 64 ? 4 - RT : DP <= 128 ? 2 : 1) void kvm_rows_kernel(const AttnArgs a)
+__global__ __launch_bounds__(DP == 256 ? 128 : 256, DP == 128 && RT == 1 ? 2 : 1) void kvm_rows_kernel(const AttnArgs a)
 {
     typedef Rows<T, SRC, DP, RT> R;
-    __shared__ __attribute__((aligned(16))) char lds[R::kLds];
+    static_assert(64 * R::kWaves == (DP == 256 ? 128 : 256), "the launch bounds are the workgroup's size");
+    __shared__ __attribute__((aligned(1024))) char lds[R::kLds];
     R rows(a, lds);
     KvStart at;
     KvTile t;
     auto first = [&]() {
         at = uniform(a.starts + blockIdx.x);
-        t = uniform(a.tiles + at.tile);
+        t = at.first;
     };
     auto piece = [&]() {
         RowWork w;
@@ -167,12 +168,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 - RT : DP <= 128 ? 2 : 1) void kv
     first();
     RowWork now = piece();
     rows.begin(now);
+    rows.begin_v(now);
     for (;;) {
         rows.run(now);
         if (at.units == 0) break;
         const RowWork next = piece();
         rows.begin(next);
         rows.finish(now);
+        rows.begin_v(next);
         now = next;
     }
     rows.finish(now);
@@ -306,7 +309,8 @@ int check_cache(const KvmStep *step, const KvmCache *c, int device, Layer *out)
 {
     if (!c || !c->k || !c->v) return refuse(KVM_EINVAL, "null pool");
     if (step->num_blocks == 0) return refuse(KVM_EINVAL, "the plan was made without a cache");
-    if (c->format != KVM_CACHE_PLAIN && c->format != KVM_CACHE_E4M3) return refuse(KVM_EINVAL, "unknown pool format %d", c->format);
+    if (c->format != step->format)
+        return refuse(KVM_EMISMATCH, "the pools are of format %d, the plan is for format %d", c->format, (int)step->format);
     if (c->dtype != step->dtype)
         return refuse(KVM_EMISMATCH, "the pools' rows are of type %d, the plan is for type %d", c->dtype, (int)step->dtype);
     if (c->num_blocks != step->num_blocks || c->block_size != step->block_size || c->num_kv_heads != step->num_kv_heads ||
@@ -416,9 +420,9 @@ template <typename T, int SRC, int DP> int launch_rows_d(const AttnArgs &a, cons
 {
     const dim3 grid((uint32_t)step->num_row_groups);
     if constexpr (DP <= 128) {
-        if (step->row_tiles == 2) kvm_rows_kernel<T, SRC, DP, 2><<<grid, 256, 0, stream>>>(a);
+        if (step->row_tiles == 2) kvm_rows_kernel<T, SRC, DP, 2><<<grid, 64 * Rows<T, SRC, DP, 2>::kWaves, 0, stream>>>(a);
     }
-    if (step->row_tiles == 1) kvm_rows_kernel<T, SRC, DP, 1><<<grid, 256, 0, stream>>>(a);
+    if (step->row_tiles == 1) kvm_rows_kernel<T, SRC, DP, 1><<<grid, 64 * Rows<T, SRC, DP, 1>::kWaves, 0, stream>>>(a);
     return check_launch("attention");
 }
 
@@ -636,6 +640,9 @@ int kvm_prompt_attention(const KvmStep *step, const int32_t *words, const KvmRow
     KV_TRY(check_rows(k, "k", step->num_tokens, step->num_kv_heads, step, device));
     KV_TRY(check_rows(v, "v", step->num_tokens, step->num_kv_heads, step, device));
     const uint64_t size = (uint64_t)type_bytes(step->dtype);
+    // the kernels step over 16 rows with 32-bit offsets
+    if ((uint64_t)k->token_stride * size >= 1u << 28 || (uint64_t)v->token_stride * size >= 1u << 28)
+        return refuse(KVM_EINVAL, "K and V rows 256 MiB apart or more are not supported");
     AttnArgs a = {};
     a.k = (const char *)k->ptr;
     a.v = (const char *)v->ptr;

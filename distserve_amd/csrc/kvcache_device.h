@@ -46,7 +46,9 @@ template <typename T> __device__ inline bool not_finite(uint32_t w)
 {
     constexpr uint32_t m = Elem<T>::kExponent;
     if constexpr (sizeof(T) == 4) return (w & m) == m;
-    return (w & m & 0xffffu) == (m & 0xffffu) || (w & m & 0xffff0000u) == (m & 0xffff0000u);
+    // 16-bit types: one more in the exponent's lowest place carries into the sign's
+    constexpr uint32_t one = std::is_same<T, _Float16>::value ? 0x04000400u : 0x00800080u;
+    return (((w & 0x7fff7fffu) + one) & 0x80008000u) != 0;
 }
 
 // ---- e4m3 codes with a power-of-two scale for each row

@@ -35,8 +35,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Sequences' sums stay in int32 (words of the plan), with room for a tile's overhang.
 constexpr int64_t kMaxTokens = (1ll << 31) - 4096;
 
-// Workgroups of the kernel for few rows that run at the same time: what its registers allow for a head_dim.
-int64_t most_groups(int64_t head_dim) { return kCus * (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1); }
+// Workgroups of the kernel for few rows that run at the same time: as many as fit the CUs' registers and LDS.
+int64_t most_groups(int64_t head_dim) { return kCus * (head_dim <= 64 ? 3 : 2); }
 
 }  // namespace
 
@@ -67,13 +67,15 @@ int64_t kvm_plan_words(int64_t num_seqs, int64_t num_tokens, int64_t num_pages, 
 
 int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t num_seqs, const int64_t *table,
                   const int64_t *table_len, int64_t num_blocks, int64_t block_size, int64_t num_heads,
-                  int64_t num_kv_heads, int64_t head_dim, int32_t dtype, int32_t *words, int64_t capacity, KvmStep *step)
+                  int64_t num_kv_heads, int64_t head_dim, int32_t dtype, int32_t format, int32_t *words, int64_t capacity,
+                  KvmStep *step)
 {
     if (!step || !words) return refuse(KVM_EINVAL, "kvm_plan_step: null output");
     if (num_seqs < 0 || (num_seqs > 0 && (!first_token || !new_tokens)))
         return refuse(KVM_EINVAL, "kvm_plan_step: bad sequence lists");
     if (dtype != KVM_F16 && dtype != KVM_BF16 && dtype != KVM_F32)
         return refuse(KVM_EINVAL, "kvm_plan_step: unknown dtype %d", dtype);
+    if (format != KVM_CACHE_PLAIN && format != KVM_CACHE_E4M3) return refuse(KVM_EINVAL, "unknown pool format %d", format);
     if (num_heads < 1 || num_kv_heads < 1 || num_heads % num_kv_heads != 0 || num_heads > (1 << 20))
         return refuse(KVM_EINVAL, "num_heads (%lld) must be a positive multiple of num_kv_heads (%lld)",
                       (long long)num_heads, (long long)num_kv_heads);
@@ -125,6 +127,7 @@ int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t
     out.head_dim = head_dim;
     out.all_new = all_new ? 1 : 0;
     out.dtype = dtype;
+    out.format = format;
 
     const int64_t slots = cached ? tokens : 0;
     out.table_at = 0;
@@ -206,7 +209,7 @@ int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t
         int64_t head = 0, unit = 0, open = -1;   // open: the group that began the pair at hand and left it unfinished
         for (int64_t w = 0; w < groups; ++w) {
             int64_t left = units / groups + (w < units % groups ? 1 : 0);
-            starts.push_back(KvStart{(int32_t)tile, (int32_t)head, (int32_t)unit, (int32_t)left});
+            starts.push_back(KvStart{tiles[tile], (int32_t)tile, (int32_t)head, (int32_t)unit, (int32_t)left});
             while (left > 0) {
                 const KvTile &t = tiles[tile];
                 const int64_t n = std::min<int64_t>(left, t.units - unit);

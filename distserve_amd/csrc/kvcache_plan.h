@@ -20,6 +20,7 @@ struct KvTile {
 // Where a workgroup of the kernel for few rows starts: the units of all (tile, KV head) pairs in a row are
 // dealt out evenly, so that every workgroup has the same amount to read.
 struct KvStart {
+    KvTile first;       // the tile it starts with
     int32_t tile, head, unit, units;
 };
 

@@ -14,7 +14,7 @@
 
 namespace kvc {
 
-// Rows row0 .. row0 + count - 1 of the piece, dealt out over the workgroup's four waves.
+// Rows row0 .. row0 + count - 1 of the piece, dealt out over the workgroup's waves.
 template <typename T, int SRC, int DP>
 __device__ __forceinline__ void attend_slow(const AttnArgs &a, const RowWork w, const int count)
 {
@@ -22,7 +22,7 @@ __device__ __forceinline__ void attend_slow(const AttnArgs &a, const RowWork w, 
     constexpr int U = SRC == kE4m3 ? 16 : 16 / (int)sizeof(T);    // elements of a 16-byte load
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int D = (int)a.head_dim;
-    for (int r = wave; r < count && w.row0 + r < w.rows; r += 4) {
+    for (int r = wave; r < count && w.row0 + r < w.rows; r += (int)blockDim.x / 64) {
         const uint32_t row = (uint32_t)(w.row0 + r), token = div_by(row, a.by_group), g = row - token * a.group;
         const int end = min(w.first + (int)token + 1, w.kv_end);
         const char *src = a.q + (uint64_t)(w.q_start + token) * a.q_token + (uint64_t)(w.head * a.group + g) * a.q_head;

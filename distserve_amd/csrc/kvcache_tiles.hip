@@ -309,7 +309,7 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
             for (int step = 0; step < kSteps; ++step) {
                 const int d = step * 16 + half * 8;
                 u32x4 w = {0, 0, 0, 0};
-                if (r < it.rows && d < D) w = *(const u32x4 *)(src + d * 2);
+                if ((r < it.rows) & (d < D)) w = *(const u32x4 *)(src + d * 2);
                 q[qt][step] = as<Frag>(w ^ a.q_sign);
             }
         }
@@ -324,7 +324,7 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
         for (int qt = 0; qt < QT; ++qt) {
             const int r = first_row + qt * 32 + col;
             const float sum = l[qt] + __shfl_xor(l[qt], 32);
-            if (r >= it.rows) continue;
+            const bool live = r < it.rows;
             if (it.part_row >= 0) {
                 const uint64_t at = (uint64_t)part_at() + (r - it.row0);
 #pragma unroll
@@ -332,14 +332,14 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int d = 32 * dt + 8 * i + 4 * half;
-                        if (d < D)
+                        if (live & (d < D))
                             *(f32x4 *)(a.part_acc + at * D + d) = f32x4{acc[qt][dt][4 * i], acc[qt][dt][4 * i + 1],
                                                                         acc[qt][dt][4 * i + 2], acc[qt][dt][4 * i + 3]};
                     }
-                if (half == 0) *(f32x2 *)(a.part_ml + at * 2) = f32x2{m[qt], sum};
+                if (live & (half == 0)) *(f32x2 *)(a.part_ml + at * 2) = f32x2{m[qt], sum};
                 continue;
             }
-            const uint32_t token = div_by((uint32_t)r, a.by_group), g = (uint32_t)r - token * a.group;
+            const uint32_t safe = (uint32_t)min(r, it.rows - 1), token = div_by(safe, a.by_group), g = safe - token * a.group;
             char *dst = a.out + (uint64_t)(it.q_start + token) * a.out_token + (uint64_t)(h * a.group + g) * a.out_head;
             const float inverse = 1.0f / sum;
             typedef typename Elem<T>::V4 V4;
@@ -349,7 +349,7 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
                 for (int i = 0; i < 4; ++i) {
                     const int d = 32 * dt + 8 * i + 4 * half;
                     const f32x4 x = {acc[qt][dt][4 * i], acc[qt][dt][4 * i + 1], acc[qt][dt][4 * i + 2], acc[qt][dt][4 * i + 3]};
-                    if (d < D) *(V4 *)(dst + d * 2) = __builtin_convertvector(x * inverse, V4);
+                    if (live & (d < D)) *(V4 *)(dst + d * 2) = __builtin_convertvector(x * inverse, V4);
                 }
         }
     }

@@ -64,7 +64,7 @@ struct StepPlan : torch::CustomClassHolder {
 
     StepPlan(std::vector<int64_t> first_token, std::vector<int64_t> new_tokens, std::vector<int64_t> table,
              std::vector<int64_t> table_len, int64_t num_blocks, int64_t block_size, int64_t num_heads,
-             int64_t num_kv_heads, int64_t head_dim, int64_t type, int64_t device)
+             int64_t num_kv_heads, int64_t head_dim, int64_t type, bool quantized, int64_t device)
         : dtype((c10::ScalarType)type)
     {
         TORCH_CHECK(first_token.size() == new_tokens.size(), "StepPlan: ", first_token.size(), " first tokens but ",
@@ -89,7 +89,7 @@ struct StepPlan : torch::CustomClassHolder {
                                                          num_kv_heads));
         check(kvm_plan_step(first_token.data(), new_tokens.data(), (int64_t)new_tokens.size(), table.data(),
                             table_len.data(), num_blocks, block_size, num_heads, num_kv_heads, head_dim, type_code(dtype),
-                            host.data(), (int64_t)host.size(), &step),
+                            quantized ? KVM_CACHE_E4M3 : KVM_CACHE_PLAIN, host.data(), (int64_t)host.size(), &step),
               "StepPlan");
         if (device < 0) return;   // a plan to look at, without a GPU
         const c10::hip::HIPGuard guard((c10::DeviceIndex)device);
@@ -278,7 +278,7 @@ KVM_TORCH_LIBRARY(KVM_CACHE_NS, m)
                 ", this op library was built for major version ", KVM_ABI_MAJOR);
     m.class_<StepPlan>("StepPlan")
         .def(torch::init<std::vector<int64_t>, std::vector<int64_t>, std::vector<int64_t>, std::vector<int64_t>, int64_t,
-                         int64_t, int64_t, int64_t, int64_t, int64_t, int64_t>())
+                         int64_t, int64_t, int64_t, int64_t, int64_t, bool, int64_t>())
         .def("num_tokens", [](const Plan &p) { return p->step.num_tokens; })
         .def("num_kv_tokens", [](const Plan &p) { return p->step.num_kv_tokens; })
         .def("workspace_bytes", [](const Plan &p) { return kvm_attention_workspace(&p->step); })

@@ -292,6 +292,7 @@ typedef struct KvmStep {
     int64_t block_size, num_heads, num_kv_heads, head_dim;
     int64_t all_new;        /* 1 when no sequence has tokens before this step's */
     int64_t dtype;          /* KVM_F16, KVM_BF16 or KVM_F32 */
+    int64_t format;         /* KVM_CACHE_PLAIN or KVM_CACHE_E4M3 */
     int64_t row_tiles;      /* 16-row tiles of a workgroup of the kernel for few rows */
     int64_t num_row_tiles, num_row_groups;   /* its row tiles, its workgroups */
     int64_t num_tile_items;                  /* work items of the kernel for many rows */
@@ -326,8 +327,8 @@ int64_t kvm_plan_words(int64_t num_seqs, int64_t num_tokens, int64_t num_pages, 
  */
 int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t num_seqs, const int64_t *table,
                   const int64_t *table_len, int64_t num_blocks, int64_t block_size, int64_t num_heads,
-                  int64_t num_kv_heads, int64_t head_dim, int32_t dtype, int32_t *words, int64_t capacity,
-                  KvmStep *step);
+                  int64_t num_kv_heads, int64_t head_dim, int32_t dtype, int32_t format, int32_t *words,
+                  int64_t capacity, KvmStep *step);
 
 /* One layer of a pool pair. */
 typedef struct KvmCache {

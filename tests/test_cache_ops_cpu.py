@@ -21,8 +21,8 @@ def pieces_of(step, words, heads):
     tiles = section(words, step.row_tiles_at, step.num_row_tiles, 8)
     height = 16 * step.row_tiles
     at = (0, 0, 0)
-    for group, (tile, head, unit, units) in enumerate(section(words, step.row_starts_at, step.num_row_groups, 4)):
-        assert (tile, head, unit) == at and units > 0          # each group goes on where the one before stopped
+    for group, (*copy, tile, head, unit, units) in enumerate(section(words, step.row_starts_at, step.num_row_groups, 12)):
+        assert (tile, head, unit) == at and units > 0 and tuple(copy) == tiles[tile]          # each group goes on where the one before stopped
         while units:
             q_start, rows, first, table_at, row0, kv_end, total, _ = tiles[tile]
             n = min(units, total - unit)
@@ -47,8 +47,8 @@ def pieces_of(step, words, heads):
     return few, many
 
 
-def plan(first, new, table, num_blocks=64, block_size=16, heads=8, kv_heads=2, head_dim=64, dtype=cabi.KVM_F16):
-    return cabi.plan_step(first, new, table, num_blocks, block_size, heads, kv_heads, head_dim, dtype)
+def plan(first, new, table, num_blocks=64, block_size=16, heads=8, kv_heads=2, head_dim=64, dtype=cabi.KVM_F16, format=cabi.KVM_CACHE_PLAIN):
+    return cabi.plan_step(first, new, table, num_blocks, block_size, heads, kv_heads, head_dim, dtype, format)
 
 
 def test_a_plan_names_every_slot_and_page():
@@ -79,7 +79,7 @@ def test_the_pieces_of_a_plan_cover_every_row_and_key_once(heads, kv_heads, head
         for p in pages:
             table.append(order[at:at + p])
             at += p
-        step, words = plan(first, new, table, len(order), 16, heads, kv_heads, head_dim, dtype)
+        step, words = plan(first, new, table, len(order), 16, heads, kv_heads, head_dim, dtype, case % 2)
         group = heads // kv_heads
         starts, table_at = [0], [0]
         for b, p in zip(new, pages):
@@ -115,7 +115,7 @@ def test_the_pieces_of_a_plan_cover_every_row_and_key_once(heads, kv_heads, head
         assert len(set(used)) == len(used) and all(0 <= r < step.part_rows for r in used)
         assert cabi.attention_workspace(step) == step.part_rows * (head_dim + 2) * 4
         # every group of the kernel for few rows has the same amount to read, give or take a unit
-        shares = [g[3] for g in section(words, step.row_starts_at, step.num_row_groups, 4)]
+        shares = [g[11] for g in section(words, step.row_starts_at, step.num_row_groups, 12)]
         assert not shares or max(shares) - min(shares) <= 1
 
 
@@ -139,7 +139,7 @@ def test_plans_refuse_what_a_kernel_could_trip_over():
     plan([16, 16], [1, 1], [[7, 8], [7, 9]])                            # a shared prefix is fine
     plan([3, 4], [1, 1], [[7], [7]])                                    # and so are two slots of one block
     for bad in (dict(heads=7), dict(heads=0), dict(kv_heads=0), dict(head_dim=72), dict(head_dim=0), dict(head_dim=272),
-                dict(dtype=3), dict(block_size=0), dict(block_size=70000), dict(num_blocks=-1),
+                dict(dtype=3), dict(format=2), dict(block_size=0), dict(block_size=70000), dict(num_blocks=-1),
                 dict(num_blocks=2**27, block_size=16)):
         refused(cabi.KVM_EINVAL, *ok, **bad)
     refused(cabi.KVM_ERANGE, [2**31], [1], [[0]])
@@ -153,7 +153,7 @@ def test_plans_refuse_what_a_kernel_could_trip_over():
     # too little room is refused, not overrun
     words, first, new = (ctypes.c_int32 * 64)(), (ctypes.c_int64 * 1)(0), (ctypes.c_int64 * 1)(40)
     table, lens, out = (ctypes.c_int64 * 3)(0, 1, 2), (ctypes.c_int64 * 1)(3), cabi.KvmStep()
-    rc = cabi.lib.kvm_plan_step(first, new, 1, table, lens, 8, 16, 8, 2, 64, 0, words, 30, ctypes.byref(out))
+    rc = cabi.lib.kvm_plan_step(first, new, 1, table, lens, 8, 16, 8, 2, 64, 0, 0, words, 30, ctypes.byref(out))
     assert rc == cabi.KVM_EINVAL and b"kvm_plan_words" in cabi.lib.kvm_last_error()
 
 
@@ -192,7 +192,7 @@ def test_the_op_layer_refuses_cpu_tensors_and_plans_without_a_gpu():
         distserve_amd.plan_step(z, [1], [0], [[0]], 4)
     with pytest.raises(RuntimeError, match="not torch.float64"):
         distserve_amd.plan_prompt([1], 2, 2, 64, torch.float64, "cuda:0")
-    held = distserve_amd.StepPlan([0], [3], [1], [1], 4, 16, 4, 2, 64, 5, -1)      # a plan to look at
+    held = distserve_amd.StepPlan([0], [3], [1], [1], 4, 16, 4, 2, 64, 5, False, -1)      # a plan to look at
     assert held.num_tokens() == 3 and held.device_index() == -1
     row = torch.zeros(3, 2, 64, dtype=torch.float16)
     with pytest.raises(RuntimeError, match="without a GPU"):
@@ -200,7 +200,7 @@ def test_the_op_layer_refuses_cpu_tensors_and_plans_without_a_gpu():
     for bad in (([0], [3], [1], [2], 4), ([0, 0], [3], [1], [1], 4), ([0], [3], [1], [], 4), ([0], [-3], [1], [1], 4),
                 ([0], [3], [4], [1], 4)):
         with pytest.raises(RuntimeError):
-            distserve_amd.StepPlan(*bad, 16, 4, 2, 64, 5, -1)
+            distserve_amd.StepPlan(*bad, 16, 4, 2, 64, 5, False, -1)
 
 
 def test_the_alternate_namespace_has_the_cache_ops_too():
@@ -213,7 +213,7 @@ def test_the_alternate_namespace_has_the_cache_ops_too():
         ours = str(getattr(torch.ops.kvcache_ops, name).default._schema)
         theirs = str(getattr(torch.ops.kvmove_kvcache_ops, name).default._schema)
         assert theirs.replace("kvmove_kvcache_ops", "kvcache_ops") == ours
-    plan = torch.classes.kvmove_kvcache_ops.StepPlan([0], [3], [1], [1], 4, 16, 4, 2, 64, 5, -1)
+    plan = torch.classes.kvmove_kvcache_ops.StepPlan([0], [3], [1], [1], 4, 16, 4, 2, 64, 5, False, -1)
     assert plan.num_kv_tokens() == 3
 
 

@@ -505,7 +505,7 @@ def test_the_c_interface_checks_extents_and_workspaces():
                        (cabi.KVM_ERANGE, (cache(num_layers=1 << 20), rows(q), rows(out), 0.125, work.data_ptr(), need, stream)),
                        (cabi.KVM_EMISMATCH, (cache(head_dim=128), rows(q), rows(out), 0.125, work.data_ptr(), need, stream)),
                        (cabi.KVM_EMISMATCH, (cache(dtype=cabi.KVM_BF16), rows(q), rows(out), 0.125, work.data_ptr(), need, stream)),
-                       (cabi.KVM_EINVAL, (cache(format=7), rows(q), rows(out), 0.125, work.data_ptr(), need, stream)),
+                       (cabi.KVM_EMISMATCH, (cache(format=cabi.KVM_CACHE_E4M3), rows(q), rows(out), 0.125, work.data_ptr(), need, stream)),
                        (cabi.KVM_EINVAL, (cache(k=0), rows(q), rows(out), 0.125, work.data_ptr(), need, stream))):
         with pytest.raises(cabi.KvmError) as e:
             cabi.paged_attention(step, dev.data_ptr(), *args)
