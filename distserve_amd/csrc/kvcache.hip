@@ -21,7 +21,8 @@ using namespace kvc;
 // ---- write and read back
 //
 // Pure data movement: a lane takes eight elements of a row, 8, 16 or 32 lanes a row (the power of two
-// that covers head_dim; lanes past it idle).  Both are bound by HBM.
+// that covers head_dim; lanes past it idle).  Both are bound by HBM.  Consecutive rows of a workgroup are
+// consecutive tokens of one head, which lie side by side in the pool (codes and, more so, their scale bytes).
 
 struct MoveArgs {
     const int32_t *slots;       // write: the new tokens' cache slots; read: {first output row, tokens} of each table entry
@@ -41,9 +42,9 @@ template <typename T, bool Q, int LANES>
 __global__ __launch_bounds__(256) void kvm_write_kernel(const MoveArgs a)
 {
     constexpr int W = sizeof(T) * 2;                                   // words of a lane's eight elements
-    const uint32_t row = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    if (row >= a.tokens * a.heads) return;                             // a row's lanes leave together
-    const uint32_t token = div_by(row, a.by_heads), head = row - token * a.heads;
+    const uint32_t group = div_by(blockIdx.x, a.by_heads), head = blockIdx.x - group * a.heads;
+    const uint32_t token = group * (256 / LANES) + threadIdx.x / LANES;
+    if (token >= a.tokens) return;                                     // a row's lanes leave together
     const bool is_v = blockIdx.y != 0;
     const uint32_t d = threadIdx.x % LANES * 8;
     const bool live = d < a.head_dim;
@@ -60,7 +61,7 @@ __global__ __launch_bounds__(256) void kvm_write_kernel(const MoveArgs a)
         if (live) {
 #pragma unroll
             for (int i = 0; i < W / 4; ++i)
-                *((u32x4 *)(slab + off * a.row_bytes + d * sizeof(T)) + i) = *(u32x4 *)(w + 4 * i);
+                __builtin_nontemporal_store(*(u32x4 *)(w + 4 * i), (u32x4 *)(slab + off * a.row_bytes + d * sizeof(T)) + i);
         }
     } else {
         float x[8], top = 0.0f;
@@ -115,6 +116,10 @@ __global__ __launch_bounds__(256) void kvm_read_kernel(const MoveArgs a)
             const float scale = power_of(*(const uint8_t *)(slab + a.codes + t));
             decode4<T>(c[0], scale, w);
             decode4<T>(c[1], scale, w + W / 2);
+            if (may_overflow<T>(scale)) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) w[i] = saturated(w[i]);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < W / 4; ++i)
@@ -388,7 +393,7 @@ constexpr uint64_t kMaxGroups = 0xffffffffull / 256;   // workgroups of 256 in a
 
 template <typename T, bool Q, int LANES> int launch_write(const MoveArgs &a, hipStream_t stream)
 {
-    const uint64_t groups = ((uint64_t)a.tokens * a.heads + 256 / LANES - 1) / (256 / LANES);
+    const uint64_t groups = ((uint64_t)a.tokens + 256 / LANES - 1) / (256 / LANES) * a.heads;
     if (2 * groups > kMaxGroups) return refuse(KVM_EINVAL, "too many rows for one launch");
     kvm_write_kernel<T, Q, LANES><<<dim3((uint32_t)groups, 2), 256, 0, stream>>>(a);
     return check_launch("kvm_write_kv");

@@ -55,21 +55,13 @@ template <typename T> __device__ inline bool not_finite(uint32_t w)
 
 __device__ inline float power_of(uint32_t byte) { return __uint_as_float(byte << 23); }   // 2^(byte-127), byte >= 1
 
-// Four codes as T, times the row's scale: exact (four significant bits), except that a code may
-// have rounded past the largest fp16 number, which it then becomes (byte >= 135 only: 448 * 2^7
-// still fits).
+// Four codes as T, times the row's scale: exact (four significant bits), but for fp16's range, which `saturated` sees to.
 template <typename T> __device__ inline void decode4(uint32_t codes, float scale, uint32_t out[])
 {
     if constexpr (std::is_same<T, _Float16>::value) {
         union { f16x2 h; uint32_t w; } a, b;
         a.h = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, false);
         b.h = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, true);
-        if (scale >= 256.0f) {
-            for (uint32_t *w : {&a.w, &b.w}) {
-                if ((*w & 0x7fffu) == 0x7c00u) *w -= 1;
-                if ((*w & 0x7fff0000u) == 0x7c000000u) *w -= 0x10000u;
-            }
-        }
         out[0] = a.w;
         out[1] = b.w;
     } else if constexpr (std::is_same<T, __bf16>::value) {
@@ -87,6 +79,17 @@ template <typename T> __device__ inline void decode4(uint32_t codes, float scale
         out[2] = b.w[0];
         out[3] = b.w[1];
     }
+}
+
+// Whether codes under this scale may be past the largest fp16 number (448 * 2^7 is not).
+template <typename T> __device__ inline bool may_overflow(float scale) { return std::is_same<T, _Float16>::value && scale >= 256.0f; }
+
+// A code may have rounded past the largest fp16 number, which it then becomes.
+__device__ inline uint32_t saturated(uint32_t w)
+{
+    if ((w & 0x7fffu) == 0x7c00u) w -= 1;
+    if ((w & 0x7fff0000u) == 0x7c000000u) w -= 0x10000u;
+    return w;
 }
 
 // Two elements of T in a word (one of float) as floats.

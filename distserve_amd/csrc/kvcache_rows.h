@@ -209,6 +209,11 @@ template <typename T, int SRC, int DP, int RT> struct Rows {
     // Codes that have arrived, as values into the wave's tile.
     __device__ __forceinline__ void decode()
     {
+        if (__builtin_expect(__any(may_overflow<T>(fmaxf(kscale, vscale))), 0)) decode_as<true>();
+        else decode_as<false>();
+    }
+    template <bool LARGE> __device__ __forceinline__ void decode_as()
+    {
 #pragma unroll
         for (int j = 0; j < kCodeLoads; ++j) {
             const int row = j * kCodeRows + lane / (DP / 16), first = lane % (DP / 16) * (16 / EF);
@@ -216,14 +221,14 @@ template <typename T, int SRC, int DP, int RT> struct Rows {
             char *at = tile() + row * kRow;
 #pragma unroll
             for (int f = 0; f < 16 / EF; ++f) {
-                *(u32x4 *)(at + ((first + f) ^ swizzle_k(row)) * 16) = values(kw[j], f, ks);
-                *(u32x4 *)(at + kHalf + ((first + f) ^ swizzle_v(row)) * 16) = values(vw[j], f, vs);
+                *(u32x4 *)(at + ((first + f) ^ swizzle_k(row)) * 16) = values<LARGE>(kw[j], f, ks);
+                *(u32x4 *)(at + kHalf + ((first + f) ^ swizzle_v(row)) * 16) = values<LARGE>(vw[j], f, vs);
             }
         }
     }
 
     // Chunk f of 16 codes.
-    static __device__ __forceinline__ u32x4 values(u32x4 w, int f, float scale)
+    template <bool LARGE> static __device__ __forceinline__ u32x4 values(u32x4 w, int f, float scale)
     {
         uint32_t t[4];
         if constexpr (sizeof(T) == 2) {
@@ -232,6 +237,7 @@ template <typename T, int SRC, int DP, int RT> struct Rows {
         } else {
             decode4<T>(w[f], scale, t);
         }
+        if constexpr (LARGE) return u32x4{saturated(t[0]), saturated(t[1]), saturated(t[2]), saturated(t[3])};
         return u32x4{t[0], t[1], t[2], t[3]};
     }
 

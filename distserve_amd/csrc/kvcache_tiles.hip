@@ -126,22 +126,31 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
     __device__ void store(int buffer)
     {
         if constexpr (SRC == kE4m3) {
-            const int row = 16 * wave + (lane >> 2);
-            char *at = lds + buffer * kTile + row * kRow;
-#pragma unroll
-            for (int j = 0; j < kCoded; ++j)
-#pragma unroll
-                for (int f = 0; f < 2; ++f) {
-                    const int chunk = (4 * j + (lane & 3)) * 2 + f;
-                    uint32_t k[4], v[4];
-                    decode4<T>(kw[j][2 * f], kscale, k);
-                    decode4<T>(kw[j][2 * f + 1], kscale, k + 2);
-                    decode4<T>(vw[j][2 * f], vscale, v);
-                    decode4<T>(vw[j][2 * f + 1], vscale, v + 2);
-                    *(u32x4 *)(at + (chunk ^ swizzle_k(row)) * 16) = u32x4{k[0], k[1], k[2], k[3]};
-                    *(u32x4 *)(at + 2 * kTile + (chunk ^ swizzle_v(row)) * 16) = u32x4{v[0], v[1], v[2], v[3]};
-                }
+            if (__builtin_expect(__any(may_overflow<T>(fmaxf(kscale, vscale))), 0)) store_as<true>(buffer);
+            else store_as<false>(buffer);
         }
+    }
+    template <bool LARGE> __device__ __forceinline__ void store_as(int buffer)
+    {
+        const int row = 16 * wave + (lane >> 2);
+        char *at = lds + buffer * kTile + row * kRow;
+#pragma unroll
+        for (int j = 0; j < kCoded; ++j)
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+                const int chunk = (4 * j + (lane & 3)) * 2 + f;
+                *(u32x4 *)(at + (chunk ^ swizzle_k(row)) * 16) = values<LARGE>(kw[j], f, kscale);
+                *(u32x4 *)(at + 2 * kTile + (chunk ^ swizzle_v(row)) * 16) = values<LARGE>(vw[j], f, vscale);
+            }
+    }
+    // Chunk f of 16 codes.
+    template <bool LARGE> static __device__ __forceinline__ u32x4 values(u32x4 w, int f, float scale)
+    {
+        uint32_t t[4];
+        decode4<T>(w[2 * f], scale, t);
+        decode4<T>(w[2 * f + 1], scale, t + 2);
+        if constexpr (LARGE) return u32x4{saturated(t[0]), saturated(t[1]), saturated(t[2]), saturated(t[3])};
+        return u32x4{t[0], t[1], t[2], t[3]};
     }
 
     Frag q[QT][kSteps];
@@ -248,7 +257,7 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
             }
     }
 
-    // All tiles; false as soon as one that is masked holds an infinity or a NaN in V, which a weight of zero does
+    // All tiles, the first of which is on its way; false as soon as one that is masked holds an infinity or a NaN in V, which a weight of zero does
     // not keep from the rows that may not see it.
     __device__ bool pass(int first_row)
     {
@@ -268,8 +277,6 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
         const int least = it.first + (int)div_by((uint32_t)it.row0, a.by_group);
         const int wave_least = it.first + (int)div_by((uint32_t)min(first_row, it.rows - 1), a.by_group);
         const int most = it.first + (int)div_by((uint32_t)max(last_row, 0), a.by_group);
-        if constexpr (SRC != kPacked) fetch_pages(0);
-        load(0, 0);
         store(0);
         for (int t = 0; t < tiles; ++t) {
             __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): the wave's share of the tile has arrived
@@ -299,6 +306,9 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
             for (int i = threadIdx.x; i < kLds / 16; i += 256) *(u32x4 *)(lds + i * 16) = u32x4{0, 0, 0, 0};
             __syncthreads();
         }
+        // the first tile, and the rows meanwhile
+        if constexpr (SRC != kPacked) fetch_pages(0);
+        load(0, 0);
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
             const int r = first_row + qt * 32 + col, clamped = min(r, it.rows - 1);
