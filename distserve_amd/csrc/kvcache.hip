@@ -37,6 +37,58 @@ struct MoveArgs {
     Divider by_heads, by_block;
 };
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+
+// Maximum over the LANES lanes of a row (8, 16 or 32): neighbours, pairs, mirrored eights and sixteens.
+template <int LANES> __device__ inline uint32_t row_max(uint32_t x)
+{
+    x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true));    // quad_perm 1 0 3 2
+    x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true));    // quad_perm 2 3 0 1
+    x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xf, 0xf, true));   // row_half_mirror
+    if constexpr (LANES >= 16) x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x140, 0xf, 0xf, true));   // row_mirror
+    if constexpr (LANES >= 32) x = max(x, (uint32_t)__shfl_xor((int)x, 16));
+    return x;
+}
+
+// The finite number whose magnitude has these bits.
+template <typename T> __device__ inline float magnitude(uint32_t bits)
+{
+    return element<T>(&bits, 0);
+}
+
+// Smallest e with top <= 448 * 2^e, -126 at least, 0 for 0; 448 = 0.875 * 2^9.
+__device__ inline int scale_exponent(float top)
+{
+    int x;
+    const float part = frexpf(top, &x);
+    return top > 0.0f ? max(part <= 0.875f ? x - 9 : x - 8, -126) : 0;
+}
+
+// Four elements divided by the scale (a power of two), as codes: rounded to nearest, ties to even.
+template <typename T> __device__ inline uint32_t encode4(const uint32_t *w, float scale)
+{
+    union { s16x2 h; uint32_t w; } c;
+    c.w = 0;
+    if constexpr (std::is_same<T, _Float16>::value) {
+        union { uint32_t w; f16x2 h; } a, b;
+        a.w = w[0];
+        b.w = w[1];
+        c.h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c.h, a.h, scale, false);
+        c.h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c.h, b.h, scale, true);
+    } else if constexpr (std::is_same<T, __bf16>::value) {
+        union { uint32_t w; bf16x2 h; } a, b;
+        a.w = w[0];
+        b.w = w[1];
+        c.h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c.h, a.h, scale, false);
+        c.h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c.h, b.h, scale, true);
+    } else {
+        c.h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c.h, __uint_as_float(w[0]), __uint_as_float(w[1]), scale, false);
+        c.h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c.h, __uint_as_float(w[2]), __uint_as_float(w[3]), scale, true);
+    }
+    return c.w;
+}
+
 // T: the rows' type.  Q: quantised pool.  LANES: lanes of a row.
 template <typename T, bool Q, int LANES>
 __global__ __launch_bounds__(256) void kvm_write_kernel(const MoveArgs a)
@@ -64,32 +116,51 @@ __global__ __launch_bounds__(256) void kvm_write_kernel(const MoveArgs a)
                 __builtin_nontemporal_store(*(u32x4 *)(w + 4 * i), (u32x4 *)(slab + off * a.row_bytes + d * sizeof(T)) + i);
         }
     } else {
-        float x[8], top = 0.0f;
+        // Largest magnitude of the row, by bit patterns: those of finite numbers are in the numbers' order, and those of
+        // infinities and NaN above them all.
+        constexpr uint32_t kInf = sizeof(T) == 4 ? 0x7f800000u : Elem<T>::kExponent & 0xffffu;
+        uint32_t top = 0;
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x[i] = element<T>(w, i);
-            top = fmaxf(top, fabsf(x[i]) < INFINITY ? fabsf(x[i]) : 0.0f);
-        }
+            for (int i = 0; i < W; ++i) top = max(top, w[i] & 0x7fffffffu);
+        } else {
+            u16x2 pair = {0, 0};
 #pragma unroll
-        for (int m = 1; m < LANES; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-        // smallest e with top <= 448 * 2^e; 448 = 0.875 * 2^9
-        int e = 0;
-        if (top > 0.0f) {
-            int x2;
-            const float part = frexpf(top, &x2);
-            e = max(part <= 0.875f ? x2 - 9 : x2 - 8, -126);
+            for (int i = 0; i < W; ++i) {
+                union { uint32_t w; u16x2 h; } x;
+                x.w = w[i] & 0x7fff7fffu;
+                pair = __builtin_elementwise_max(pair, x.h);
+            }
+            top = max((uint32_t)pair[0], (uint32_t)pair[1]);
         }
-        const float inverse = power_of((uint32_t)(127 - e));          // e <= 120, so this is a normal number
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float y = x[i] * inverse;
-            x[i] = y != y ? y : fminf(fmaxf(y, -448.0f), 448.0f);
-        }
+        top = row_max<LANES>(top);
         uint32_t c[2];
+        int e;
+        if (__builtin_expect(!__any(top >= kInf), 1)) {
+            e = scale_exponent(magnitude<T>(top));
+            const float scale = power_of((uint32_t)(127 + e));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            int p = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
-            c[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], p, true);
+            for (int i = 0; i < 2; ++i) c[i] = encode4<T>(w + i * W / 2, scale);
+        } else {
+            // infinities do not count for the scale and saturate; NaN stays NaN
+            float x[8], most = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = element<T>(w, i);
+                most = fmaxf(most, fabsf(x[i]) < INFINITY ? fabsf(x[i]) : 0.0f);
+            }
+            e = scale_exponent(__uint_as_float(row_max<LANES>(__float_as_uint(most))));
+            const float inverse = power_of((uint32_t)(127 - e));          // e <= 120, so this is a normal number
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = x[i] * inverse;
+                x[i] = y != y ? y : fminf(fmaxf(y, -448.0f), 448.0f);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int p = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
+                c[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], p, true);
+            }
         }
         if (live) *(u32x2 *)(slab + off * a.row_bytes + d) = u32x2{c[0], c[1]};
         if (d == 0) *(uint8_t *)(slab + a.codes + off) = (uint8_t)(e + 127);
