@@ -10,6 +10,7 @@
 #include "kvcache_slow.h"
 #include "kvcache_tiles.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -541,7 +542,8 @@ int attend(const KvmStep *step, const int32_t *words, AttnArgs a, int format, co
                           (long long)(workspace ? workspace_bytes : 0), (long long)need);
         KV_TRY(check_memory(step, workspace, (uint64_t)need, workspace_bytes, "the workspace", &device));
     }
-    if ((uint64_t)(step->num_tile_items * step->num_kv_heads) > kMaxGroups || (uint64_t)step->num_joins * 16 > kMaxGroups)
+    const uint64_t tile_groups = (uint64_t)(step->num_tile_items * std::min(step->num_kv_heads, kHeadBlock));
+    if (tile_groups > kMaxGroups || (uint64_t)step->num_joins * 16 > kMaxGroups)
         return refuse(KVM_EINVAL, "too many rows for one launch");
     const uint64_t size = (uint64_t)type_bytes(step->dtype);
     a.table = words + step->table_at;
@@ -573,7 +575,7 @@ int attend(const KvmStep *step, const int32_t *words, AttnArgs a, int format, co
     a.starts = (const KvStart *)(words + step->row_starts_at);
     a.items = (const KvItem *)(words + step->tile_items_at);
     if (step->num_tile_items > 0)
-        KV_TRY(kvm_launch_tiles(a, (int)step->dtype, format, (uint32_t)(step->num_tile_items * step->num_kv_heads), stream));
+        KV_TRY(kvm_launch_tiles(a, (int)step->dtype, format, (uint32_t)tile_groups, stream));
     if (step->num_row_groups > 0) {
         if (format == kPacked) KV_TRY(launch_rows_t<kPacked>(a, step, stream));
         else if (format == kE4m3) KV_TRY(launch_rows_t<kE4m3>(a, step, stream));

@@ -62,7 +62,7 @@ int64_t kvm_plan_words(int64_t num_seqs, int64_t num_tokens, int64_t num_pages, 
     const int64_t tiles = num_seqs + num_tokens * group / 16;            // one at least for each sequence
     const int64_t big = num_seqs + num_tokens * group / kTileRows;
     return 64 + num_pages * 3 + num_tokens + tiles * kTileWords + most_groups(16) * (kStartWords + kJoinWords) +
-           (2 * big + kTileTarget) * kItemWords + big * num_kv_heads * kJoinWords;
+           (2 * big + kTileTarget) * ceil_div(num_kv_heads, kHeadBlock) * kItemWords + big * num_kv_heads * kJoinWords;
 }
 
 int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t num_seqs, const int64_t *table,
@@ -234,41 +234,61 @@ int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t
     }
     out.row_part_rows = joins.empty() ? 0 : 2 * groups * tile_rows;
 
-    // many rows: 128-row tiles, their keys cut where that spreads the step over the chip
+    // Many rows: 128-row tiles, their keys cut where that spreads the step over the chip.  Long pieces come first, so that
+    // the last workgroups to start are short (chunks among decoding steps, 8 KV heads: 152 us, 164 us by sequence).  With more
+    // KV heads than a block has, the tiles of a sequence follow each other for a block's heads at a time instead, so that
+    // each die's L2 keeps the one head's K and V that its workgroups read in turn (16 prompts, 32 heads: 367 us, 392 us by length).
     std::vector<KvItem> items;
+    std::vector<int64_t> big;
+    std::vector<int64_t> row_of((size_t)num_seqs), table_of((size_t)num_seqs);
     int64_t keys = 0, part = 0;
-    for (int64_t s = 0; s < num_seqs; ++s)
-        for (int64_t r = 0; in_tiles(s) && r < new_tokens[s] * group; r += kTileRows)
-            keys += first_token[s] + (std::min(r + kTileRows, new_tokens[s] * group) - 1) / group + 1;
-    const int64_t piece = std::max(ceil_div(ceil_div(keys * num_kv_heads, kTileTarget), kTileStep) * kTileStep, kMinTilePiece);
-    std::vector<KvJoin> cut;
     q_start = table_at = 0;
     for (int64_t s = 0; s < num_seqs; ++s) {
+        row_of[(size_t)s] = q_start;
+        table_of[(size_t)s] = table_at;
+        q_start += new_tokens[s];
+        if (cached) table_at += table_len[s];
+        if (!in_tiles(s)) continue;
+        big.push_back(s);
+        for (int64_t r = 0; r < new_tokens[s] * group; r += kTileRows)
+            keys += first_token[s] + (std::min(r + kTileRows, new_tokens[s] * group) - 1) / group + 1;
+    }
+    std::stable_sort(big.begin(), big.end(),
+                     [&](int64_t a, int64_t b) { return first_token[a] + new_tokens[a] > first_token[b] + new_tokens[b]; });
+    const int64_t piece = std::max(ceil_div(ceil_div(keys * num_kv_heads, kTileTarget), kTileStep) * kTileStep, kMinTilePiece);
+    std::vector<KvJoin> cut;
+    for (int64_t s : big) {
         const int64_t rows = new_tokens[s] * group;
-        for (int64_t r = 0; in_tiles(s) && r < rows; r += kTileRows) {
+        const size_t begin = items.size();
+        for (int64_t r = (rows - 1) / kTileRows * kTileRows; r >= 0; r -= kTileRows) {
             const int64_t here = std::min(kTileRows, rows - r);
             const int64_t end = first_token[s] + (r + here - 1) / group + 1;
             const int64_t cuts = std::max<int64_t>(1, end / piece + (end % piece > piece / 2 ? 1 : 0));
             const int64_t len = ceil_div(ceil_div(end, cuts), kTileStep) * kTileStep;
             const int64_t pieces = ceil_div(end, len);
             for (int64_t p = 0; p < pieces; ++p)
-                items.push_back(KvItem{(int32_t)q_start, (int32_t)rows, (int32_t)first_token[s], (int32_t)table_at, (int32_t)r,
-                                       (int32_t)(p * len), (int32_t)std::min(end, (p + 1) * len),
-                                       pieces > 1 ? (int32_t)(part + p * here) : -1});
+                items.push_back(KvItem{(int32_t)row_of[(size_t)s], (int32_t)rows, (int32_t)first_token[s],
+                                       (int32_t)table_of[(size_t)s], (int32_t)r, (int32_t)(p * len),
+                                       (int32_t)std::min(end, (p + 1) * len), pieces > 1 ? (int32_t)(part + p * here) : -1, 0, 0, 0, 0});
             if (pieces > 1) {
-                cut.push_back(KvJoin{(int32_t)q_start, (int32_t)r, (int32_t)here, 0, (int32_t)part, (int32_t)(part + here),
+                cut.push_back(KvJoin{(int32_t)row_of[(size_t)s], (int32_t)r, (int32_t)here, 0, (int32_t)part, (int32_t)(part + here),
                                      (int32_t)here, (int32_t)pieces});
                 part += pieces * here;
                 join_rows = std::max(join_rows, here);
             }
             if (part * num_kv_heads > kMaxTokens) return refuse(KVM_EINVAL, "a step of more than 2^31 partial rows is not supported");
         }
-        q_start += new_tokens[s];
-        if (cached) table_at += table_len[s];
+        const size_t end = items.size();
+        for (int64_t head0 = kHeadBlock; head0 < num_kv_heads; head0 += kHeadBlock)
+            for (size_t i = begin; i < end; ++i) {
+                KvItem it = items[i];
+                it.head0 = (int32_t)head0;
+                items.push_back(it);
+            }
     }
-    // the longest pieces first, so that the last workgroups to start are short
-    std::stable_sort(items.begin(), items.end(),
-                     [](const KvItem &a, const KvItem &b) { return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin; });
+    if (num_kv_heads <= kHeadBlock)
+        std::stable_sort(items.begin(), items.end(),
+                         [](const KvItem &a, const KvItem &b) { return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin; });
     out.item_part_rows = part;
     out.part_rows = out.row_part_rows + part * num_kv_heads;
     if (out.part_rows > kMaxTokens) return refuse(KVM_EINVAL, "a step of more than 2^31 partial rows is not supported");

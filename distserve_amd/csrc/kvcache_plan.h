@@ -24,11 +24,13 @@ struct KvStart {
     int32_t tile, head, unit, units;
 };
 
-// A piece of attention work for the kernel for many rows, for every KV head: rows row0 .. over keys [kv_begin, kv_end).
+// A piece of attention work for the kernel for many rows: rows row0 .. over keys [kv_begin, kv_end), for KV heads
+// head0 .. head0 + kHeadBlock - 1 (those that exist).
 struct KvItem {
     int32_t q_start, rows, first, table_at, row0;   // as above
     int32_t kv_begin, kv_end;
     int32_t part_row;   // first partial row of this piece for KV head 0, -1 when the piece is the whole row
+    int32_t head0, pad0, pad1, pad2;
 };
 
 // Rows of one KV head whose keys were cut into pieces: partial rows start at part_row, then at next_row + i * pitch.
@@ -49,6 +51,7 @@ constexpr int64_t kTileRows = 128;            // of a workgroup of the kernel fo
 constexpr int64_t kTileStep = 64;             // keys of its tiles
 constexpr int64_t kTileTarget = 1024;         // workgroups it is cut into at least, if the pieces stay above
 constexpr int64_t kMinTilePiece = 512;        // this many keys
+constexpr int64_t kHeadBlock = 8;             // KV heads side by side: one for each of the chip's eight dies, which have an L2 each
 
 uint64_t kvm_step_seal(const KvmStep &s);
 

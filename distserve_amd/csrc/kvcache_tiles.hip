@@ -39,7 +39,8 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
     static constexpr int kRow = DP * 2;                 // bytes of a row in LDS
     static constexpr int kChunks = DP / 8;
     static constexpr int kTile = kKeys * kRow;
-    static constexpr int kLds = 4 * kTile;              // K, K, V, V
+    static constexpr int kFlags = 4 * kTile;            // K, K, V, V, then whether a wave saw an infinity or a NaN, twice
+    static constexpr int kLds = kFlags + 32;
     static constexpr int kSteps = DP / 16;              // k steps of the first product
     static constexpr int kDt = DP / 32;                 // 32-wide tiles of head_dim in the output
     static constexpr int kRowsPerLoad = 1024 / kRow;    // rows of a wave's 16-byte-a-lane load
@@ -47,6 +48,7 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
     static constexpr int kCoded = DP / 64;              // quantised: 16-code loads of a lane for a row
 
     static __device__ int swizzle_k(int row) { return DP == 64 ? (row >> 1) & 7 : row & 15; }
+    static __device__ int swizzle_out(int row) { return DP == 64 ? row & 7 : row & 15; }
     static __device__ int swizzle_v(int row) { return DP == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2; }
 
     const AttnArgs &a;
@@ -279,19 +281,26 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
         const int most = it.first + (int)div_by((uint32_t)max(last_row, 0), a.by_group);
         store(0);
         for (int t = 0; t < tiles; ++t) {
-            __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): the wave's share of the tile has arrived
-            __syncthreads();                      // and so has everybody's; nobody reads the other buffer any more
-            if (t + 1 < tiles) load(t + 1, (t + 1) & 1);
             const int base = it.kv_begin + t * kKeys, end = base + kKeys - 1;
-            if (end > least && __syncthreads_or(odd_values(t & 1))) return false;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the wave's share of the tile has arrived
+            int *flags = (int *)(lds + kFlags) + (t & 1) * 4;
+            if (end > least) {
+                const bool odd = __any(odd_values(t & 1));
+                if (lane == 0) flags[wave] = odd;
+            }
+            __syncthreads();                      // everybody's has; nobody reads the other buffer any more
+            if (t + 1 < tiles) load(t + 1, (t + 1) & 1);
+            if (end > least) {
+                if (__builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3])) return false;
+            }
             if (!idle && base <= most) compute(base, t & 1, end > wave_least);
             if (t + 1 < tiles) store((t + 1) & 1);
         }
         return true;
     }
 
-    __device__ TileKernel(const AttnArgs &args, char *shared, uint32_t item_id, uint32_t head)
-        : a(args), it(uniform(args.items + item_id)), h((int)head), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
+    __device__ TileKernel(const AttnArgs &args, char *shared, const KvItem &item, uint32_t head)
+        : a(args), it(item), h(item.head0 + (int)head), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
           lane(threadIdx.x & 63), col(threadIdx.x & 31), half((threadIdx.x & 63) >> 5), lds(shared)
     {
     }
@@ -303,7 +312,7 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
     {
         const int D = (int)a.head_dim, first_row = it.row0 + wave * QT * 32;
         if (D < DP) {
-            for (int i = threadIdx.x; i < kLds / 16; i += 256) *(u32x4 *)(lds + i * 16) = u32x4{0, 0, 0, 0};
+            for (int i = threadIdx.x; i < kFlags / 16; i += 256) *(u32x4 *)(lds + i * 16) = u32x4{0, 0, 0, 0};
             __syncthreads();
         }
         // the first tile, and the rows meanwhile
@@ -330,6 +339,7 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
             __builtin_amdgcn_s_waitcnt(0x0f70);   // the next tile may still be on its way into LDS
             return;
         }
+        __syncthreads();   // the tiles have been read
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
             const int r = first_row + qt * 32 + col;
@@ -349,18 +359,25 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
                 if (live & (half == 0)) *(f32x2 *)(a.part_ml + at * 2) = f32x2{m[qt], sum};
                 continue;
             }
-            const uint32_t safe = (uint32_t)min(r, it.rows - 1), token = div_by(safe, a.by_group), g = safe - token * a.group;
-            char *dst = a.out + (uint64_t)(it.q_start + token) * a.out_token + (uint64_t)(h * a.group + g) * a.out_head;
+            // the wave's rows through its share of the tiles, so that whole rows are written at a time
+            char *mine = lds + wave * kTile;
             const float inverse = 1.0f / sum;
             typedef typename Elem<T>::V4 V4;
 #pragma unroll
             for (int dt = 0; dt < kDt; ++dt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int d = 32 * dt + 8 * i + 4 * half;
                     const f32x4 x = {acc[qt][dt][4 * i], acc[qt][dt][4 * i + 1], acc[qt][dt][4 * i + 2], acc[qt][dt][4 * i + 3]};
-                    if (live & (d < D)) *(V4 *)(dst + d * 2) = __builtin_convertvector(x * inverse, V4);
+                    *(V4 *)(mine + col * kRow + ((4 * dt + i) ^ swizzle_out(col)) * 16 + half * 8) = __builtin_convertvector(x * inverse, V4);
                 }
+#pragma unroll
+            for (int j = 0; j < 2 * kLoads; ++j) {
+                const int row = j * kRowsPerLoad + lane / kChunks, chunk = lane % kChunks, to = first_row + qt * 32 + row;
+                const u32x4 x = *(const u32x4 *)(mine + row * kRow + (chunk ^ swizzle_out(row)) * 16);
+                const uint32_t safe = (uint32_t)min(to, it.rows - 1), token = div_by(safe, a.by_group), g = safe - token * a.group;
+                char *dst = a.out + (uint64_t)(it.q_start + token) * a.out_token + (uint64_t)(h * a.group + g) * a.out_head;
+                if ((to < it.rows) & (chunk * 8 < D)) *(u32x4 *)(dst + chunk * 16) = x;
+            }
         }
     }
 };
@@ -370,9 +387,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kvm_tiles_kernel(const
 {
     typedef TileKernel<T, SRC, DP, QT> K;
     __shared__ __attribute__((aligned(1024))) char lds[K::kLds];
-    const uint32_t item_id = div_by(blockIdx.x, a.by_heads);
-    K kernel(a, lds, item_id, blockIdx.x - item_id * a.heads);
-    kernel.run();
+    const uint32_t width = min(a.heads, (uint32_t)kHeadBlock);
+    const uint32_t item_id = a.heads < kHeadBlock ? div_by(blockIdx.x, a.by_heads) : blockIdx.x / (uint32_t)kHeadBlock;
+    K kernel(a, lds, uniform(a.items + item_id), blockIdx.x - item_id * width);
+    if (kernel.h < (int)a.heads) kernel.run();
 }
 
 template <typename T, int SRC> void launch(const AttnArgs &a, uint32_t groups, hipStream_t stream)

@@ -36,14 +36,11 @@ def pieces_of(step, words, heads):
                     head, tile = 0, tile + 1
         at = (tile, head, unit)
     assert at == (step.num_row_tiles, 0, 0)                    # and nothing is left over
-    lengths = []
-    for q_start, rows, first, table_at, row0, kv0, kv1, part in section(words, step.tile_items_at, step.num_tile_items, 8):
-        assert kv0 % 64 == 0
-        lengths.append(kv1 - kv0)
-        for head in range(heads):
+    for q_start, rows, first, table_at, row0, kv0, kv1, part, head0, *_ in section(words, step.tile_items_at, step.num_tile_items, 12):
+        assert kv0 % 64 == 0 and head0 % 8 == 0
+        for head in range(head0, min(heads, head0 + 8)):
             at_head = -1 if part < 0 else step.row_part_rows + head * step.item_part_rows + part
             many.setdefault((q_start, row0, head), []).append((kv0, kv1, at_head))
-    assert lengths == sorted(lengths, reverse=True)
     return few, many
 
 
@@ -87,8 +84,8 @@ def test_the_pieces_of_a_plan_cover_every_row_and_key_once(heads, kv_heads, head
             table_at.append(table_at[-1] + p)
         tile_of = [128 if dtype != cabi.KVM_F32 and m * group > 32 else 16 * step.row_tiles for m in new]
         # the tiles' and items' own fields
-        for at, count in ((step.row_tiles_at, step.num_row_tiles), (step.tile_items_at, step.num_tile_items)):
-            for q_start, total, begin, table_start, row0, *_ in section(words, at, count, 8):
+        for at, count, width in ((step.row_tiles_at, step.num_row_tiles, 8), (step.tile_items_at, step.num_tile_items, 12)):
+            for q_start, total, begin, table_start, row0, *_ in section(words, at, count, width):
                 s = next(s for s in range(n) if starts[s] == q_start and new[s] > 0)
                 assert total == new[s] * group and begin == first[s] and table_start == table_at[s]
                 assert (tile_of[s] == 128) == (at == step.tile_items_at) and row0 % tile_of[s] == 0
