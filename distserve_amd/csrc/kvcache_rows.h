@@ -108,6 +108,11 @@ template <typename T, int SRC, int DP, int RT> struct Rows {
         : a(args), lds(shared), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), lane(threadIdx.x & 63),
           col(threadIdx.x & 15), quarter((threadIdx.x & 63) >> 4)
     {
+        // chunks of K past head_dim are never loaded: they stay as they are here
+        if ((int)a.head_dim < DP) {
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) *(u32x4 *)(tile() + j * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
+        }
     }
 
     __device__ __forceinline__ char *tile() { return lds + wave * kTile; }
@@ -191,17 +196,22 @@ template <typename T, int SRC, int DP, int RT> struct Rows {
     // Codes of the tile start on their way into registers.
     __device__ __forceinline__ void load_codes(const RowWork &w, int base)
     {
-        const bool together = in_a_row<kCodeRows>(w, base);
+        const int row = lane / (DP / 16), d = lane % (DP / 16) * 16;
+        uint64_t at[kCodeLoads];
+        if (in_a_row<kCodeRows>(w, base)) {
 #pragma unroll
-        for (int j = 0; j < kCodeLoads; ++j) {
-            const int row = lane / (DP / 16), d = lane % (DP / 16) * 16;
-            uint64_t at;
-            if (together) at = of_first_row(k_off, j * kCodeRows) + row * a.row_bytes + d;
-            else at = of_row(k_off, j * kCodeRows + row) + d;
-            kw[j] = vw[j] = u32x4{0, 0, 0, 0};
-            if (d < (int)a.head_dim) {
-                kw[j] = __builtin_nontemporal_load((const u32x4 *)(a.k + at));
-                vw[j] = __builtin_nontemporal_load((const u32x4 *)(a.v + at));
+            for (int j = 0; j < kCodeLoads; ++j) at[j] = of_first_row(k_off, j * kCodeRows) + (row * a.row_bytes + d);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kCodeLoads; ++j) at[j] = of_row(k_off, j * kCodeRows + row) + d;
+        }
+#pragma unroll
+        for (int j = 0; j < kCodeLoads; ++j) kw[j] = vw[j] = u32x4{0, 0, 0, 0};
+        if (d < (int)a.head_dim) {
+#pragma unroll
+            for (int j = 0; j < kCodeLoads; ++j) {
+                kw[j] = __builtin_nontemporal_load((const u32x4 *)(a.k + at[j]));
+                vw[j] = __builtin_nontemporal_load((const u32x4 *)(a.v + at[j]));
             }
         }
     }
@@ -340,8 +350,7 @@ template <typename T, int SRC, int DP, int RT> struct Rows {
 #pragma unroll
             for (int j = 0; j < NF; ++j) {
                 const int row = s * 16 + col, chunk = 4 * j + quarter;
-                u32x4 x = *(const u32x4 *)(tile() + row * kRow + (chunk ^ swizzle_k(row)) * 16);
-                if ((int)a.head_dim < DP && chunk * EF >= (int)a.head_dim) x = u32x4{0, 0, 0, 0};   // not loaded
+                const u32x4 x = *(const u32x4 *)(tile() + row * kRow + (chunk ^ swizzle_k(row)) * 16);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) sc[rt][s] = mma(as<Frag>(x), q[rt][j], sc[rt][s]);
             }
@@ -385,8 +394,10 @@ template <typename T, int SRC, int DP, int RT> struct Rows {
                 p4[rt][s] = __builtin_convertvector(sc[rt][s], typename Elem<T>::V4);
             }
             l[rt] = l[rt] * alpha + sum;
+            if (__any(alpha != 1.0f)) {
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) acc[rt][dt] *= alpha;
+                for (int dt = 0; dt < DT; ++dt) acc[rt][dt] *= alpha;
+            }
         }
 
         // O^T += V^T P^T
