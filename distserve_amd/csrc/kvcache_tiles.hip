@@ -1,7 +1,7 @@
 // kvcache_tiles.hip -- attention of many query rows (chunks of prompts, whole prompts), 16-bit types.
 //
-// A workgroup of four waves takes QT*128 query rows (tokens x the group's heads) of one KV head over
-// the keys of its item, 64 keys at a time; a wave has QT*32 of the rows.  As in the row kernel,
+// A workgroup of four waves takes 128 query rows (tokens x the group's heads) of one KV head over
+// the keys of its item, 64 keys at a time; a wave has 32 of the rows.  As in the row kernel,
 // S^T = K Q^T and O^T = V^T P^T, so that a query row is a lane column of both products (32x32x16
 // matrix instructions; lanes l and l+32 share the row) and P^T needs no shuffle between them.
 //
@@ -34,7 +34,7 @@ __device__ inline f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_am
 
 __device__ inline float max_halves(float x) { return fmaxf(x, __shfl_xor(x, 32)); }
 
-template <typename T, int SRC, int DP, int QT> struct TileKernel {
+template <typename T, int SRC, int DP> struct TileKernel {
     typedef typename Elem<T>::Frag Frag;
     static constexpr int kRow = DP * 2;                 // bytes of a row in LDS
     static constexpr int kChunks = DP / 8;
@@ -155,10 +155,10 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
         return u32x4{t[0], t[1], t[2], t[3]};
     }
 
-    Frag q[QT][kSteps];
-    f32x16 acc[QT][kDt];
-    float m[QT], l[QT];    // maximum (scaled, in powers of two) that the weights refer to; the lane's share of their sum
-    int limit[QT];
+    Frag q[kSteps];
+    f32x16 acc[kDt];
+    float m, l;    // maximum (scaled, in powers of two) that the weights refer to; the lane's share of their sum
+    int limit;
 
     // Whether the wave's 16 rows of the V tile hold an infinity or a NaN: exponents of all ones carry into the
     // sign's place.
@@ -179,70 +179,64 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
     __device__ void compute(int base, int buffer, bool masked)
     {
         const char *kt = lds + buffer * kTile, *vt = kt + 2 * kTile;
-        f32x16 s[QT][2];
+        f32x16 s[2];
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[qt][u][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int step = 0; step < kSteps; ++step) {
                 const int row = 32 * u + col;
                 const Frag kf = *(const Frag *)(kt + row * kRow + (((2 * step + half) ^ swizzle_k(row)) << 4));
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt) s[qt][u] = mma(kf, q[qt][step], s[qt][u]);
+                s[u] = mma(kf, q[step], s[u]);
             }
-        Frag p[QT][4];
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-            if (masked) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (base + 32 * u + 8 * (i / 4) + 4 * half + i % 4 > limit[qt]) s[qt][u][i] = -INFINITY;
-            }
-            float top = -INFINITY;
+        Frag p[4];
+        if (masked) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[qt][u][i]);
-            top = max_halves(top) * a.scale_log2;
-            // The weights may refer to an older maximum as long as they stay below 2^8 (fp16 holds 2^15): rescaling
-            // the accumulators is then rare.
-            if (__any(top > m[qt] + 8.0f)) {
-                const float m_new = fmaxf(m[qt], top);
-                const float alpha = m[qt] == -INFINITY ? 0.0f : exp2_of(m[qt] - m_new);
-                m[qt] = m_new;
-                l[qt] *= alpha;
+                for (int i = 0; i < 16; ++i)
+                    if (base + 32 * u + 8 * (i / 4) + 4 * half + i % 4 > limit) s[u][i] = -INFINITY;
+        }
+        float top = -INFINITY;
 #pragma unroll
-                for (int dt = 0; dt < kDt; ++dt)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[qt][dt][i] *= alpha;
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
+        top = max_halves(top) * a.scale_log2;
+        // The weights may refer to an older maximum as long as they stay below 2^8 (fp16 holds 2^15): rescaling
+        // the accumulators is then rare.
+        if (__any(top > m + 8.0f)) {
+            const float m_new = fmaxf(m, top);
+            const float alpha = m == -INFINITY ? 0.0f : exp2_of(m - m_new);
+            m = m_new;
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
+        }
+        const float safe = m == -INFINITY ? 0.0f : m;   // nothing seen yet: weights of zero, not NaN
+        float sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float w = exp2_of(fmaf(s[u][i], a.scale_log2, -safe));
+                s[u][i] = w;
+                sum += w;
             }
-            const float safe = m[qt] == -INFINITY ? 0.0f : m[qt];   // nothing seen yet: weights of zero, not NaN
-            float sum = 0.0f;
+        l += sum;
+        // weights are rounded to T for the product: half a step of T each, against 32-bit sums
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+        for (int k = 0; k < 4; ++k) {
+            typedef float f32x8 __attribute__((ext_vector_type(8)));
+            f32x8 w;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float w = exp2_of(fmaf(s[qt][u][i], a.scale_log2, -safe));
-                    s[qt][u][i] = w;
-                    sum += w;
-                }
-            l[qt] += sum;
-            // weights are rounded to T for the product: half a step of T each, against 32-bit sums
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                typedef float f32x8 __attribute__((ext_vector_type(8)));
-                f32x8 w;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = s[qt][k / 2][8 * (k % 2) + i];
-                p[qt][k] = __builtin_convertvector(w, Frag);
-            }
+            for (int i = 0; i < 8; ++i) w[i] = s[k / 2][8 * (k % 2) + i];
+            p[k] = __builtin_convertvector(w, Frag);
         }
         // O^T += V^T P^T; slot (half, e) of a k step stands for key 16*k + 8*(e/4) + 4*half + e%4
         const int rr = (lane & 15) >> 2, part = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
@@ -254,8 +248,7 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
                 union { s16x4 h[2]; u32x4 w; } vf;
                 vf.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)at);
                 vf.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(at + 8 * kRow));
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt) acc[qt][dt] = mma(as<Frag>(vf.w), p[qt][k], acc[qt][dt]);
+                acc[dt] = mma(as<Frag>(vf.w), p[k], acc[dt]);
             }
     }
 
@@ -263,18 +256,15 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
     // not keep from the rows that may not see it.
     __device__ bool pass(int first_row)
     {
+        m = -INFINITY;
+        l = 0.0f;
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-            m[qt] = -INFINITY;
-            l[qt] = 0.0f;
+        for (int dt = 0; dt < kDt; ++dt)
 #pragma unroll
-            for (int dt = 0; dt < kDt; ++dt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[qt][dt][i] = 0.0f;
-        }
+            for (int i = 0; i < 16; ++i) acc[dt][i] = 0.0f;
         const int tiles = (it.kv_end - it.kv_begin + kKeys - 1) / kKeys;
         // the first row sees keys up to `least`; the wave's first row up to `wave_least`, its last one up to `most`
-        const int last_row = min(first_row + QT * 32, it.rows) - 1;
+        const int last_row = min(first_row + 32, it.rows) - 1;
         const bool idle = first_row >= it.rows;
         const int least = it.first + (int)div_by((uint32_t)it.row0, a.by_group);
         const int wave_least = it.first + (int)div_by((uint32_t)min(first_row, it.rows - 1), a.by_group);
@@ -310,7 +300,7 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
 
     __device__ void run()
     {
-        const int D = (int)a.head_dim, first_row = it.row0 + wave * QT * 32;
+        const int D = (int)a.head_dim, first_row = it.row0 + wave * 32;
         if (D < DP) {
             for (int i = threadIdx.x; i < kFlags / 16; i += 256) *(u32x4 *)(lds + i * 16) = u32x4{0, 0, 0, 0};
             __syncthreads();
@@ -318,74 +308,67 @@ template <typename T, int SRC, int DP, int QT> struct TileKernel {
         // the first tile, and the rows meanwhile
         if constexpr (SRC != kPacked) fetch_pages(0);
         load(0, 0);
+        const int r = first_row + col, clamped = min(r, it.rows - 1);
+        const uint32_t token = div_by((uint32_t)clamped, a.by_group), g = (uint32_t)clamped - token * a.group;
+        limit = min(it.first + (int)token, it.kv_end - 1);
+        const char *src = a.q + (uint64_t)(it.q_start + token) * a.q_token + (uint64_t)(h * a.group + g) * a.q_head;
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-            const int r = first_row + qt * 32 + col, clamped = min(r, it.rows - 1);
-            const uint32_t token = div_by((uint32_t)clamped, a.by_group), g = (uint32_t)clamped - token * a.group;
-            limit[qt] = min(it.first + (int)token, it.kv_end - 1);
-            const char *src = a.q + (uint64_t)(it.q_start + token) * a.q_token + (uint64_t)(h * a.group + g) * a.q_head;
-#pragma unroll
-            for (int step = 0; step < kSteps; ++step) {
-                const int d = step * 16 + half * 8;
-                u32x4 w = {0, 0, 0, 0};
-                if ((r < it.rows) & (d < D)) w = *(const u32x4 *)(src + d * 2);
-                q[qt][step] = as<Frag>(w ^ a.q_sign);
-            }
+        for (int step = 0; step < kSteps; ++step) {
+            const int d = step * 16 + half * 8;
+            u32x4 w = {0, 0, 0, 0};
+            if ((r < it.rows) & (d < D)) w = *(const u32x4 *)(src + d * 2);
+            q[step] = as<Frag>(w ^ a.q_sign);
         }
         if (!pass(first_row)) {
             const RowWork all = {it.q_start, it.rows, it.first, it.table_at, it.row0, h, it.kv_begin, it.kv_end,
                                  it.part_row < 0 ? -1 : part_at()};
-            attend_slow<T, SRC, DP>(a, all, QT * 128);
+            attend_slow<T, SRC, DP>(a, all, 128);
             __builtin_amdgcn_s_waitcnt(0x0f70);   // the next tile may still be on its way into LDS
             return;
         }
         __syncthreads();   // the tiles have been read
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-            const int r = first_row + qt * 32 + col;
-            const float sum = l[qt] + __shfl_xor(l[qt], 32);
-            const bool live = r < it.rows;
-            if (it.part_row >= 0) {
-                const uint64_t at = (uint64_t)part_at() + (r - it.row0);
-#pragma unroll
-                for (int dt = 0; dt < kDt; ++dt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int d = 32 * dt + 8 * i + 4 * half;
-                        if (live & (d < D))
-                            *(f32x4 *)(a.part_acc + at * D + d) = f32x4{acc[qt][dt][4 * i], acc[qt][dt][4 * i + 1],
-                                                                        acc[qt][dt][4 * i + 2], acc[qt][dt][4 * i + 3]};
-                    }
-                if (live & (half == 0)) *(f32x2 *)(a.part_ml + at * 2) = f32x2{m[qt], sum};
-                continue;
-            }
-            // the wave's rows through its share of the tiles, so that whole rows are written at a time
-            char *mine = lds + wave * kTile;
-            const float inverse = 1.0f / sum;
-            typedef typename Elem<T>::V4 V4;
+        const float sum = l + __shfl_xor(l, 32);
+        const bool live = r < it.rows;
+        if (it.part_row >= 0) {
+            const uint64_t at = (uint64_t)part_at() + (r - it.row0);
 #pragma unroll
             for (int dt = 0; dt < kDt; ++dt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const f32x4 x = {acc[qt][dt][4 * i], acc[qt][dt][4 * i + 1], acc[qt][dt][4 * i + 2], acc[qt][dt][4 * i + 3]};
-                    *(V4 *)(mine + col * kRow + ((4 * dt + i) ^ swizzle_out(col)) * 16 + half * 8) = __builtin_convertvector(x * inverse, V4);
+                    const int d = 32 * dt + 8 * i + 4 * half;
+                    if (live & (d < D))
+                        *(f32x4 *)(a.part_acc + at * D + d) = f32x4{acc[dt][4 * i], acc[dt][4 * i + 1],
+                                                                    acc[dt][4 * i + 2], acc[dt][4 * i + 3]};
                 }
+            if (live & (half == 0)) *(f32x2 *)(a.part_ml + at * 2) = f32x2{m, sum};
+            return;
+        }
+        // the wave's rows through its share of the tiles, so that whole rows are written at a time
+        char *mine = lds + wave * kTile;
+        const float inverse = 1.0f / sum;
+        typedef typename Elem<T>::V4 V4;
 #pragma unroll
-            for (int j = 0; j < 2 * kLoads; ++j) {
-                const int row = j * kRowsPerLoad + lane / kChunks, chunk = lane % kChunks, to = first_row + qt * 32 + row;
-                const u32x4 x = *(const u32x4 *)(mine + row * kRow + (chunk ^ swizzle_out(row)) * 16);
-                const uint32_t safe = (uint32_t)min(to, it.rows - 1), token = div_by(safe, a.by_group), g = safe - token * a.group;
-                char *dst = a.out + (uint64_t)(it.q_start + token) * a.out_token + (uint64_t)(h * a.group + g) * a.out_head;
-                if ((to < it.rows) & (chunk * 8 < D)) *(u32x4 *)(dst + chunk * 16) = x;
+        for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 x = {acc[dt][4 * i], acc[dt][4 * i + 1], acc[dt][4 * i + 2], acc[dt][4 * i + 3]};
+                *(V4 *)(mine + col * kRow + ((4 * dt + i) ^ swizzle_out(col)) * 16 + half * 8) = __builtin_convertvector(x * inverse, V4);
             }
+#pragma unroll
+        for (int j = 0; j < 2 * kLoads; ++j) {
+            const int row = j * kRowsPerLoad + lane / kChunks, chunk = lane % kChunks, to = first_row + row;
+            const u32x4 x = *(const u32x4 *)(mine + row * kRow + (chunk ^ swizzle_out(row)) * 16);
+            const uint32_t safe = (uint32_t)min(to, it.rows - 1), token = div_by(safe, a.by_group), g = safe - token * a.group;
+            char *dst = a.out + (uint64_t)(it.q_start + token) * a.out_token + (uint64_t)(h * a.group + g) * a.out_head;
+            if ((to < it.rows) & (chunk * 8 < D)) *(u32x4 *)(dst + chunk * 16) = x;
         }
     }
 };
 
-template <typename T, int SRC, int DP, int QT>
+template <typename T, int SRC, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kvm_tiles_kernel(const AttnArgs a)
 {
-    typedef TileKernel<T, SRC, DP, QT> K;
+    typedef TileKernel<T, SRC, DP> K;
     __shared__ __attribute__((aligned(1024))) char lds[K::kLds];
     const uint32_t width = min(a.heads, (uint32_t)kHeadBlock);
     const uint32_t item_id = a.heads < kHeadBlock ? div_by(blockIdx.x, a.by_heads) : blockIdx.x / (uint32_t)kHeadBlock;
@@ -395,9 +378,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kvm_tiles_kernel(const
 
 template <typename T, int SRC> void launch(const AttnArgs &a, uint32_t groups, hipStream_t stream)
 {
-    if (a.head_dim <= 64) kvm_tiles_kernel<T, SRC, 64, 1><<<groups, 256, 0, stream>>>(a);
-    else if (a.head_dim <= 128) kvm_tiles_kernel<T, SRC, 128, 1><<<groups, 256, 0, stream>>>(a);
-    else kvm_tiles_kernel<T, SRC, 256, 1><<<groups, 256, 0, stream>>>(a);
+    if (a.head_dim <= 64) kvm_tiles_kernel<T, SRC, 64><<<groups, 256, 0, stream>>>(a);
+    else if (a.head_dim <= 128) kvm_tiles_kernel<T, SRC, 128><<<groups, 256, 0, stream>>>(a);
+    else kvm_tiles_kernel<T, SRC, 256><<<groups, 256, 0, stream>>>(a);
 }
 
 template <typename T> void launch_source(const AttnArgs &a, int source, uint32_t groups, hipStream_t stream)
