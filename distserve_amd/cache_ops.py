@@ -16,6 +16,8 @@ tokens one after the other; slices of a fused projection are fine (any token and
 strides that keep rows at multiples of 16 bytes).  Tensors may have more rows than the step has
 tokens (a batch padded to a fixed size): those behind the last sequence are neither read nor
 written (a new output holds zeros there).
+An ``out`` may be a slice of the tensor that q is a slice of, but must not share memory with what the call
+reads; the K and the V pool of a write must be two.  Such calls are refused.
 
 A pool is plain, ``[num_blocks, layers, kv_heads, block_size, head_dim]`` of the rows' type, or
 quantised: uint8 with last dimension ``head_dim + 1`` (``quantized_pool_shape``), e4m3 codes with a

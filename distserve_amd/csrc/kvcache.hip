@@ -416,6 +416,13 @@ int check_cache(const KvmStep *step, const KvmCache *c, int device, Layer *out)
     return KVM_OK;
 }
 
+// Elements from the first to behind the last one.
+unsigned __int128 reach(const KvmRows *r, int64_t tokens, int64_t heads, int64_t head_dim)
+{
+    return (unsigned __int128)(tokens - 1) * (uint64_t)r->token_stride + (unsigned __int128)(heads - 1) * (uint64_t)r->head_stride +
+           (uint64_t)head_dim;
+}
+
 int check_rows(const KvmRows *r, const char *what, int64_t tokens, int64_t heads, const KvmStep *step, int device)
 {
     const int64_t size = type_bytes(step->dtype);
@@ -424,8 +431,9 @@ int check_rows(const KvmRows *r, const char *what, int64_t tokens, int64_t heads
     if ((uintptr_t)r->ptr % 16 != 0 || r->token_stride * size % 16 != 0 || r->head_stride * size % 16 != 0)
         return refuse(KVM_EINVAL, "%s: rows must start at multiples of 16 bytes (strides %lld and %lld elements)", what,
                       (long long)r->token_stride, (long long)r->head_stride);
-    const uint64_t need = (uint64_t)((tokens - 1) * r->token_stride + (heads - 1) * r->head_stride + step->head_dim) * (uint64_t)size;
-    return check_memory(step, r->ptr, need, r->extent, what, &device);
+    const unsigned __int128 need = reach(r, tokens, heads, step->head_dim) * (uint64_t)size;
+    if (need > (uint64_t)INT64_MAX) return refuse(KVM_ERANGE, "%s: strides %lld and %lld are too large", what, (long long)r->token_stride, (long long)r->head_stride);
+    return check_memory(step, r->ptr, (uint64_t)need, r->extent, what, &device);
 }
 
 // Output rows of different (token, head) must not share memory.
@@ -437,6 +445,47 @@ int check_apart(const KvmRows *r, const char *what, int64_t tokens, int64_t head
         return refuse(KVM_EINVAL, "%s: rows overlap (strides %lld and %lld elements)", what, (long long)r->token_stride,
                       (long long)r->head_stride);
     return KVM_OK;
+}
+
+bool disjoint(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes)
+{
+    return (uintptr_t)a + a_bytes <= (uintptr_t)b || (uintptr_t)b + b_bytes <= (uintptr_t)a;
+}
+
+// Written rows must not lie on rows that the same call reads or writes elsewhere: workgroups come to them in any order.  Rows
+// that take turns in memory (slices of one fused projection) are apart.
+int check_clear(const KvmRows *out, int64_t out_heads, const KvmRows *in, int64_t in_heads, int64_t tokens, const KvmStep *step,
+                const char *what)
+{
+    const uint64_t size = (uint64_t)type_bytes(step->dtype), row = (uint64_t)step->head_dim * size;
+    if (disjoint(out->ptr, (uint64_t)reach(out, tokens, out_heads, step->head_dim) * size, in->ptr,
+                 (uint64_t)reach(in, tokens, in_heads, step->head_dim) * size))
+        return KVM_OK;
+    // both repeat every `period` bytes: `a` bytes of it are out's, from its start, and `b` bytes in's
+    auto take_turns = [&](uint64_t period, uint64_t a, uint64_t b) {
+        if (period == 0 || a > period || b > period) return false;
+        const uint64_t off = ((uintptr_t)in->ptr % period + period - (uintptr_t)out->ptr % period) % period;
+        return off >= a && off + b <= period;
+    };
+    auto width = [&](const KvmRows *r, int64_t heads) { return (uint64_t)(heads - 1) * (uint64_t)r->head_stride * size + row; };
+    if (out->token_stride == in->token_stride &&
+        take_turns((uint64_t)out->token_stride * size, width(out, out_heads), width(in, in_heads)))
+        return KVM_OK;
+    const int64_t head = out_heads > 1 ? out->head_stride : in->head_stride;
+    if (head > 0 && (out_heads == 1 || out->head_stride == head) && (in_heads == 1 || in->head_stride == head) &&
+        out->token_stride % head == 0 && in->token_stride % head == 0 && take_turns((uint64_t)head * size, row, row))
+        return KVM_OK;
+    return refuse(KVM_EINVAL, "%s share memory", what);
+}
+
+// The same for rows and whole pools.
+int check_clear_of_pools(const KvmRows *rows, int64_t tokens, int64_t heads, const KvmStep *step, const KvmCache *c, const Layer &layer,
+                         const char *what)
+{
+    const uint64_t bytes = layer.block_stride * (uint64_t)c->num_blocks;
+    const uint64_t need = (uint64_t)reach(rows, tokens, heads, step->head_dim) * (uint64_t)type_bytes(step->dtype);
+    if (disjoint(rows->ptr, need, c->k, bytes) && disjoint(rows->ptr, need, c->v, bytes)) return KVM_OK;
+    return refuse(KVM_EINVAL, "%s and a pool share memory", what);
 }
 
 // The device the operands are on is the current one while a call launches.
@@ -535,6 +584,7 @@ int attend(const KvmStep *step, const int32_t *words, AttnArgs a, int format, co
     KV_TRY(check_rows(q, "q", step->num_tokens, step->num_heads, step, device));
     KV_TRY(check_rows(out, "out", step->num_tokens, step->num_heads, step, device));
     KV_TRY(check_apart(out, "out", step->num_tokens, step->num_heads, step->head_dim));
+    KV_TRY(check_clear(out, step->num_heads, q, step->num_heads, step->num_tokens, step, "out and q"));
     const int64_t need = kvm_attention_workspace(step);
     if (need > 0) {
         if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16 != 0)
@@ -612,6 +662,10 @@ int kvm_write_kv(const KvmStep *step, const int32_t *words, const KvmCache *cach
     KV_TRY(check_cache(step, cache, device, &layer));
     KV_TRY(check_rows(k, "k", step->num_tokens, step->num_kv_heads, step, device));
     KV_TRY(check_rows(v, "v", step->num_tokens, step->num_kv_heads, step, device));
+    KV_TRY(check_clear_of_pools(k, step->num_tokens, step->num_kv_heads, step, cache, layer, "k"));
+    KV_TRY(check_clear_of_pools(v, step->num_tokens, step->num_kv_heads, step, cache, layer, "v"));
+    const uint64_t pool = layer.block_stride * (uint64_t)cache->num_blocks;
+    if (!disjoint(cache->k, pool, cache->v, pool)) return refuse(KVM_EINVAL, "the K pool and the V pool share memory");
     if (step->num_tokens * step->num_kv_heads > INT32_MAX) return refuse(KVM_EINVAL, "too many rows for one launch");
     const uint64_t size = (uint64_t)type_bytes(step->dtype);
     MoveArgs a = {};
@@ -656,6 +710,9 @@ int kvm_read_kv(const KvmStep *step, const int32_t *words, const KvmCache *cache
     KV_TRY(check_rows(v_out, "v_out", step->num_kv_tokens, step->num_kv_heads, step, device));
     KV_TRY(check_apart(k_out, "k_out", step->num_kv_tokens, step->num_kv_heads, step->head_dim));
     KV_TRY(check_apart(v_out, "v_out", step->num_kv_tokens, step->num_kv_heads, step->head_dim));
+    KV_TRY(check_clear(k_out, step->num_kv_heads, v_out, step->num_kv_heads, step->num_kv_tokens, step, "k_out and v_out"));
+    KV_TRY(check_clear_of_pools(k_out, step->num_kv_tokens, step->num_kv_heads, step, cache, layer, "k_out"));
+    KV_TRY(check_clear_of_pools(v_out, step->num_kv_tokens, step->num_kv_heads, step, cache, layer, "v_out"));
     if (step->num_pages * step->num_kv_heads > INT32_MAX) return refuse(KVM_EINVAL, "too many blocks for one launch");
     const uint64_t size = (uint64_t)type_bytes(step->dtype);
     MoveArgs a = {};
@@ -696,6 +753,8 @@ int kvm_paged_attention(const KvmStep *step, const int32_t *words, const KvmCach
     KV_TRY(check_words(step, words, &device));
     Layer layer;
     KV_TRY(check_cache(step, cache, device, &layer));
+    KV_TRY(check_rows(out, "out", step->num_tokens, step->num_heads, step, device));
+    KV_TRY(check_clear_of_pools(out, step->num_tokens, step->num_heads, step, cache, layer, "out"));
     AttnArgs a = {};
     a.k = layer.k;
     a.v = layer.v;
@@ -721,6 +780,9 @@ int kvm_prompt_attention(const KvmStep *step, const int32_t *words, const KvmRow
     // the kernels step over 16 rows with 32-bit offsets
     if ((uint64_t)k->token_stride * size >= 1u << 28 || (uint64_t)v->token_stride * size >= 1u << 28)
         return refuse(KVM_EINVAL, "K and V rows 256 MiB apart or more are not supported");
+    KV_TRY(check_rows(out, "out", step->num_tokens, step->num_heads, step, device));
+    KV_TRY(check_clear(out, step->num_heads, k, step->num_kv_heads, step->num_tokens, step, "out and k"));
+    KV_TRY(check_clear(out, step->num_heads, v, step->num_kv_heads, step->num_tokens, step, "out and v"));
     AttnArgs a = {};
     a.k = (const char *)k->ptr;
     a.v = (const char *)v->ptr;

@@ -16,6 +16,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <vector>
 
 namespace {
@@ -57,7 +58,10 @@ extern "C" {
 
 int64_t kvm_plan_words(int64_t num_seqs, int64_t num_tokens, int64_t num_pages, int64_t num_heads, int64_t num_kv_heads)
 {
-    if (num_seqs < 0 || num_tokens < 0 || num_pages < 0 || num_heads < 1 || num_kv_heads < 1) return KVM_EINVAL;
+    // what a plan may have at most, so that the sum below stays in 64 bits
+    if (num_seqs < 0 || num_tokens < 0 || num_pages < 0 || std::max({num_seqs, num_tokens, num_pages}) > INT32_MAX ||
+        num_heads < 1 || num_heads > (1 << 20) || num_kv_heads < 1 || num_kv_heads > num_heads)
+        return refuse(KVM_EINVAL, "kvm_plan_words: a step of that size is not supported");
     const int64_t group = std::max<int64_t>(1, num_heads / num_kv_heads);
     const int64_t tiles = num_seqs + num_tokens * group / 16;            // one at least for each sequence
     const int64_t big = num_seqs + num_tokens * group / kTileRows;
@@ -69,7 +73,7 @@ int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t
                   const int64_t *table_len, int64_t num_blocks, int64_t block_size, int64_t num_heads,
                   int64_t num_kv_heads, int64_t head_dim, int32_t dtype, int32_t format, int32_t *words, int64_t capacity,
                   KvmStep *step)
-{
+try {
     if (!step || !words) return refuse(KVM_EINVAL, "kvm_plan_step: null output");
     if (num_seqs < 0 || (num_seqs > 0 && (!first_token || !new_tokens)))
         return refuse(KVM_EINVAL, "kvm_plan_step: bad sequence lists");
@@ -204,6 +208,7 @@ int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t
         if (cached) table_at += table_len[s];
     }
     const int64_t groups = std::min(most_groups(head_dim), ceil_div(units, kMinUnits));
+    if (groups > 0 && units / groups >= INT32_MAX) return refuse(KVM_EINVAL, "a step of more than 2^31 units of keys a workgroup is not supported");
     {
         size_t tile = 0;
         int64_t head = 0, unit = 0, open = -1;   // open: the group that began the pair at hand and left it unfinished
@@ -324,6 +329,8 @@ int kvm_plan_step(const int64_t *first_token, const int64_t *new_tokens, int64_t
     out.device = -1;
     *step = out;
     return KVM_OK;
+} catch (const std::exception &e) {   // out of memory: nothing is thrown through the C interface
+    return refuse(KVM_EINVAL, "kvm_plan_step: %s", e.what());
 }
 
 int64_t kvm_attention_workspace(const KvmStep *step)

@@ -85,8 +85,9 @@ struct StepPlan : torch::CustomClassHolder {
         TORCH_CHECK(tokens <= INT32_MAX && num_heads >= 1 && num_heads <= (1 << 20) && num_kv_heads >= 1,
                     "StepPlan: ", tokens, " tokens of ", num_heads, " heads, ", num_kv_heads, " KV heads");
         TORCH_CHECK(tokens * num_heads <= ((int64_t)1 << 40), "StepPlan: too many rows");
-        std::vector<int32_t> host((size_t)kvm_plan_words((int64_t)new_tokens.size(), tokens, (int64_t)table.size(), num_heads,
-                                                         num_kv_heads));
+        const int64_t most = kvm_plan_words((int64_t)new_tokens.size(), tokens, (int64_t)table.size(), num_heads, num_kv_heads);
+        if (most < 0) check((int)most, "StepPlan");
+        std::vector<int32_t> host((size_t)most);
         check(kvm_plan_step(first_token.data(), new_tokens.data(), (int64_t)new_tokens.size(), table.data(),
                             table_len.data(), num_blocks, block_size, num_heads, num_kv_heads, head_dim, type_code(dtype),
                             quantized ? KVM_CACHE_E4M3 : KVM_CACHE_PLAIN, host.data(), (int64_t)host.size(), &step),

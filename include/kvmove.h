@@ -348,13 +348,14 @@ typedef struct KvmRows {
 } KvmRows;
 
 /* K and V of the step's new tokens into the blocks the plan names.  `words` is the device
- * copy of the plan.  Slots the step does not name are left as they are. */
+ * copy of the plan.  Slots the step does not name are left as they are.  k and v must not lie in the
+ * pools, nor the pools on each other (KVM_EINVAL). */
 int kvm_write_kv(const KvmStep *step, const int32_t *words, const KvmCache *cache, const KvmRows *k,
                  const KvmRows *v, void *stream);
 
 /* All tokens of the step's sequences (the earlier ones and the new ones), packed one
  * sequence after the other: k_out and v_out are [num_kv_tokens, num_kv_heads, head_dim] of the
- * plan's type.  Values of a quantised pool beyond the largest KVM_F16 number become that number. */
+ * plan's type, apart from each other and the pools.  Values of a quantised pool beyond the largest KVM_F16 number become that number. */
 int kvm_read_kv(const KvmStep *step, const int32_t *words, const KvmCache *cache, const KvmRows *k_out,
                 const KvmRows *v_out, void *stream);
 
@@ -371,6 +372,7 @@ int64_t kvm_attention_workspace(const KvmStep *step);
  * Tokens behind the last sequence's in q and out are neither read nor written.  Cache slots
  * that no row may attend to (blocks' unused tails, later tokens) do not reach the result,
  * whatever they hold.  Sums, maxima and accumulators are 32-bit.
+ * out may lie between q's rows in memory (slices of one wider row), not on them, nor in the pools.
  */
 int kvm_paged_attention(const KvmStep *step, const int32_t *words, const KvmCache *cache, const KvmRows *q,
                         const KvmRows *out, float scale, void *workspace, int64_t workspace_bytes, void *stream);

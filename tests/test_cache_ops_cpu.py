@@ -181,6 +181,67 @@ def test_entry_points_refuse_before_they_touch_a_device():
     cabi.paged_attention(empty, 0, pools, rows, rows, 1.0)
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are made up: only for a machine where nothing can be launched")
+def test_entry_points_refuse_memory_that_is_written_and_used():
+    step, _ = plan([0], [3], [[0]], num_blocks=4)          # 3 tokens, 8 heads, 2 KV heads of 64 in fp16: rows of 128 bytes
+    step.device = 0                                        # the caller vouches for extents: no question to the runtime
+    K, V, Q, O, S, W = (i << 24 for i in range(1, 7))
+    pool = 4 * 2 * 2 * 16 * 64 * 2
+
+    def pools(k=K, v=V):
+        return cabi.KvmCache(k, v, 4, 2, 0, 2, 16, 64, cabi.KVM_F16, cabi.KVM_CACHE_PLAIN, pool)
+
+    def rows(at, token, head=64, extent=1 << 20):
+        return cabi.KvmRows(at, token, head, extent)
+
+    def refused(code, text, call, *args):
+        with pytest.raises(cabi.KvmError, match=text) as e:
+            call(step, W, *args)
+        assert e.value.code == code, e.value
+
+    q, k, v = rows(Q, 512), rows(S, 128), rows(S + 4096, 128)
+    for out in (rows(Q, 512), rows(Q + 128, 512), rows(Q + 2048, 512), rows(Q, 1024), rows(Q + 1024, 1024 + 64),
+                rows(Q + 128, 64, 3 * 64), rows(Q - 1024 + 128, 512)):
+        refused(cabi.KVM_EINVAL, "out and q share memory", cabi.paged_attention, pools(), q, out, 1.0)
+    refused(cabi.KVM_EINVAL, "out and a pool", cabi.paged_attention, pools(), q, rows(V + pool - 16, 512), 1.0)
+    refused(cabi.KVM_EINVAL, "out and a pool", cabi.paged_attention, pools(), q, rows(K - 16, 512), 1.0)
+    refused(cabi.KVM_EINVAL, "out and k", cabi.prompt_attention, q, k, v, rows(S - 2048, 512), 1.0)
+    refused(cabi.KVM_EINVAL, "out and v", cabi.prompt_attention, q, k, rows(O + 1024, 128), rows(O, 512), 1.0)
+    refused(cabi.KVM_EINVAL, "k and a pool", cabi.write_kv, pools(), rows(K, 128), v)
+    refused(cabi.KVM_EINVAL, "v and a pool", cabi.write_kv, pools(), k, rows(K + pool - 128, 128))
+    refused(cabi.KVM_EINVAL, "the K pool and the V pool", cabi.write_kv, pools(v=K), k, v)
+    refused(cabi.KVM_EINVAL, "the K pool and the V pool", cabi.write_kv, pools(v=K + pool - 16), k, v)
+    refused(cabi.KVM_EINVAL, "k_out and v_out", cabi.read_kv, pools(), rows(O, 128), rows(O, 128))
+    refused(cabi.KVM_EINVAL, "k_out and v_out", cabi.read_kv, pools(), rows(O, 256), rows(O + 128, 256))
+    refused(cabi.KVM_EINVAL, "k_out and a pool", cabi.read_kv, pools(), rows(K + 256, 128), rows(O, 128))
+    # strides whose reach passes 64 bits
+    refused(cabi.KVM_ERANGE, "too large", cabi.write_kv, pools(), rows(S, 1 << 62), v)
+    refused(cabi.KVM_ERANGE, "too large", cabi.paged_attention, pools(), q, rows(O, 1 << 62), 1.0)
+
+
+def test_a_plan_that_memory_does_not_suffice_for_is_refused():
+    code = """
+import ctypes, resource
+from distserve_amd import cabi
+now = int(open('/proc/self/statm').read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (now + (64 << 20), now + (64 << 20)))
+try:
+    cabi.plan_step([0], [1], [[0]], 1 << 26, 31, 8, 2, 64, cabi.KVM_F16)       # a bit for each of 2^31 slots
+except cabi.KvmError as e:
+    assert e.code == cabi.KVM_EINVAL and 'alloc' in str(e), e
+    print('refused')
+"""
+    import subprocess
+    import sys
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0 and done.stdout == "refused\n", (done.returncode, done.stdout, done.stderr)
+
+
+def test_the_words_of_impossible_steps_are_refused():
+    for bad in ((-1, 1, 1, 8, 2), (1, 1 << 40, 1, 8, 2), (1, 1, 1 << 40, 8, 2), (1, 1, 1, 8, 9), (1, 1, 1, 1 << 21, 1), (1, 1, 1, 8, 0)):
+        assert cabi.lib.kvm_plan_words(*bad) == cabi.KVM_EINVAL
+
+
 def test_the_op_layer_refuses_cpu_tensors_and_plans_without_a_gpu():
     import distserve_amd
 

@@ -480,6 +480,28 @@ def test_refusals():
     assert torch.equal(out, prompt_attention(prompt, q, shared.contiguous(), shared.contiguous()))
 
 
+def test_outputs_that_lie_on_inputs_are_refused_and_fused_ones_are_not():
+    case = Case(torch.float16, "plain", 4, 2, 64, 16, [20, 300], [3, 40], seed=1)
+    kc, vc, plan = case.k_cache, case.v_cache, case.plan
+    q = case.q.cuda()
+    wide = torch.zeros(43, 12, 64, dtype=torch.float16, device="cuda")           # q, out and others in one row
+    wide[:, :4] = q
+    side = torch.zeros(43, 4, 2, 64, dtype=torch.float16, device="cuda")         # q and out in turns, head by head
+    side[:, :, 0] = q
+    row = torch.zeros(43, 2, 64, dtype=torch.float16, device="cuda")
+    for rows, out in ((q, q), (wide[:, :4], wide[:, :4]), (wide[:, :4], wide[:, 3:7]), (side[:, :, 0], side[:, :, 0])):
+        with pytest.raises(RuntimeError, match="share memory"):
+            paged_attention(plan, 1, rows, kc, vc, out=out)
+    for call in (lambda: write_kv(plan, 1, row, row, kc, kc), lambda: write_kv(plan, 1, kc.view(-1, 2, 64)[:43], row, kc, vc)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            call()
+    want = paged_attention(plan, 1, q, kc, vc)
+    assert torch.equal(paged_attention(plan, 1, wide[:, :4], kc, vc, out=wide[:, 4:8]), want)
+    assert torch.equal(paged_attention(plan, 1, side[:, :, 0], kc, vc, out=side[:, :, 1]), want)
+    assert torch.equal(wide[:, 4:8], want) and torch.equal(side[:, :, 1], want) and not wide[:, 8:].any()
+    assert torch.equal(wide[:, :4], q) and torch.equal(side[:, :, 0], q)
+
+
 def test_the_c_interface_checks_extents_and_workspaces():
     case = Case(torch.float16, "plain", 2, 2, 64, 16, [3000], [1], seed=1)
     step, words = cabi.plan_step(case.first, case.new, case.table, case.k_cache.shape[0], 16, 2, 2, 64, cabi.KVM_F16)
