@@ -14,6 +14,14 @@
 
 namespace kvc {
 
+// A decoded value as a T holds it: past the largest fp16 number it is that number.
+template <typename T> __device__ __forceinline__ float held(uint32_t w)
+{
+    const float x = __uint_as_float(w);
+    if constexpr (std::is_same<T, _Float16>::value) return fabsf(x) > 65504.0f ? copysignf(65504.0f, x) : x;
+    return x;
+}
+
 // Rows row0 .. row0 + count - 1 of the piece, dealt out over the workgroup's waves.
 template <typename T, int SRC, int DP>
 __device__ __forceinline__ void attend_slow(const AttnArgs &a, const RowWork w, const int count)
@@ -67,7 +75,7 @@ __device__ __forceinline__ void attend_slow(const AttnArgs &a, const RowWork w, 
                     for (int j = 0; j < EL; ++j)
                         if ((d + i) / 64 == j) qd = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(q[j]), (d + i) % 64));
                     float k;
-                    if constexpr (SRC == kE4m3) k = __uint_as_float(e[i]);
+                    if constexpr (SRC == kE4m3) k = held<T>(e[i]);
                     else k = element<T>(e, i);
                     s = fmaf(k, qd, s);
                 }
@@ -99,7 +107,7 @@ __device__ __forceinline__ void attend_slow(const AttnArgs &a, const RowWork w, 
                     if constexpr (SRC == kE4m3) {
                         uint32_t four[4];
                         decode4<float>(*(const uint8_t *)(a.v + off + d), scale, four);
-                        v = __uint_as_float(four[0]);
+                        v = held<T>(four[0]);
                     } else {
                         v = (float)*(const T *)(a.v + off + d * sizeof(T));
                     }

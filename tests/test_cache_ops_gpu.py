@@ -319,6 +319,26 @@ def test_a_quantised_nan_reaches_only_the_rows_that_see_it():
 
 # ---- how a program calls them
 
+@pytest.mark.parametrize("new", [3, 64])
+def test_codes_past_fp16_beside_a_nan_are_the_largest_number(new):
+    """Keys 0..5 hold 448 * 2^8 in V's column 3, which fp16 does not; the last key holds a NaN in column 5."""
+    table, last = [3, 1, 4, 2, 0], 5 + new - 1
+    kc = torch.zeros(5, 1, 1, 16, 65, dtype=torch.uint8)
+    kc.view(5, 16 * 65)[:, 16 * 64:] = 127                                    # scales of one
+    vc = kc.clone()
+    for key in range(6):
+        vc.view(5, 16 * 65)[table[0], key * 64 + 3] = 0x7e
+        vc.view(5, 16 * 65)[table[0], 16 * 64 + key] = 127 + 8
+    vc.view(5, 16 * 65)[table[last // 16], last % 16 * 64 + 5] = 0x7f
+    kc, vc = kc.cuda(), vc.cuda()
+    plan = plan_step(kc, [new], [5], [table], 1)
+    got = paged_attention(plan, 0, torch.zeros(new, 1, 64, dtype=torch.float16, device="cuda"), kc, vc).cpu()[:, 0].double()
+    want = 65504.0 * 6 / (6 + torch.arange(new, dtype=torch.float64))         # all scores are zero: plain means
+    # one rounding to fp16 (half a step, 2^-11), and sums and a quotient in 32 bits
+    assert ((got[:, 3] - want).abs() <= want * 2.0**-10).all()
+    assert got[:-1].isfinite().all() and got[-1, 5].isnan() and got[-1, :5].isfinite().all()
+
+
 def test_padded_batches_and_given_outputs_keep_what_lies_behind():
     case = Case(torch.bfloat16, "plain", 8, 2, 128, 16, [50, 0], [1, 30], seed=6)
     n = case.tokens
