@@ -545,7 +545,8 @@ template <typename T, bool Q> int launch_read_q(const MoveArgs &a, uint64_t page
 template <typename T, int SRC, int DP> int launch_rows_d(const AttnArgs &a, const KvmStep *step, hipStream_t stream)
 {
     const dim3 grid((uint32_t)step->num_row_groups);
-    if constexpr (DP <= 128) {
+    // (more than 16 rows of 16 bits over codes are the kernel for many rows' work: quantised blocks hold 16 tokens or more)
+    if constexpr (DP <= 128 && (SRC != kE4m3 || sizeof(T) == 4)) {
         if (step->row_tiles == 2) kvm_rows_kernel<T, SRC, DP, 2><<<grid, 64 * Rows<T, SRC, DP, 2>::kWaves, 0, stream>>>(a);
     }
     if (step->row_tiles == 1) kvm_rows_kernel<T, SRC, DP, 1><<<grid, 64 * Rows<T, SRC, DP, 1>::kWaves, 0, stream>>>(a);

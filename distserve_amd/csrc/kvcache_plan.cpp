@@ -36,7 +36,9 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Sequences' sums stay in int32 (words of the plan), with room for a tile's overhang.
 constexpr int64_t kMaxTokens = (1ll << 31) - 4096;
 
-// Workgroups of the kernel for few rows that run at the same time: as many as fit the CUs' registers and LDS.
+// Workgroups of the kernel for few rows: as many as run at the same time, by the CUs' registers and LDS.  Fewer leave memory
+// waiting, more only add joins (us, head_dim 128, 1, 2 and 4 a CU: 96.7, 89.0, 89.5 for 32 sequences of 1000, 32 heads, 110, 109,
+// 112 for 8 of 20000, 8 heads; head_dim 64, 2, 3 and 4: 27.0, 24.9, 28.6 for 64 of 600, 12 heads).
 int64_t most_groups(int64_t head_dim) { return kCus * (head_dim <= 64 ? 3 : 2); }
 
 }  // namespace
@@ -207,7 +209,7 @@ try {
         q_start += new_tokens[s];
         if (cached) table_at += table_len[s];
     }
-    const int64_t groups = std::min(most_groups(head_dim), ceil_div(units, kMinUnits));
+    const int64_t groups = std::min(most_groups(head_dim), units);
     if (groups > 0 && units / groups >= INT32_MAX) return refuse(KVM_EINVAL, "a step of more than 2^31 units of keys a workgroup is not supported");
     {
         size_t tile = 0;
@@ -260,7 +262,8 @@ try {
     }
     std::stable_sort(big.begin(), big.end(),
                      [&](int64_t a, int64_t b) { return first_token[a] + new_tokens[a] > first_token[b] + new_tokens[b]; });
-    const int64_t piece = std::max(ceil_div(ceil_div(keys * num_kv_heads, kTileTarget), kTileStep) * kTileStep, kMinTilePiece);
+    const int64_t all = keys * num_kv_heads, fill = std::min(std::max(ceil_div(all, kTileFill), kShortPiece), kLongPiece);
+    const int64_t piece = ceil_div(std::max(ceil_div(all, kTileTarget), fill), kTileStep) * kTileStep;
     std::vector<KvJoin> cut;
     for (int64_t s : big) {
         const int64_t rows = new_tokens[s] * group;

@@ -45,12 +45,20 @@ constexpr int64_t kJoinWords = sizeof(KvJoin) / 4;
 
 constexpr int64_t kUnit = 128;                // keys the four waves of a workgroup for few rows take in one turn
 constexpr int64_t kCus = 256;
-constexpr int64_t kMinUnits = 2;              // a workgroup for few rows takes at least, so that the joins stay few
-constexpr int64_t kFewRows = 32;              // up to here a sequence's rows go to the kernel for few rows
+// Up to here a sequence's rows go to the kernel for few rows.  16 sequences of 2048, 8 KV heads of 128, fp16, in us: 16 rows 31.8
+// there, 42.7 in the kernel for many; 24 rows 55.2 and 49.8; 32 heads of 1000 keys, 24 rows 79 and 56.
+constexpr int64_t kFewRows = 16;
 constexpr int64_t kTileRows = 128;            // of a workgroup of the kernel for many rows
 constexpr int64_t kTileStep = 64;             // keys of its tiles
-constexpr int64_t kTileTarget = 1024;         // workgroups it is cut into at least, if the pieces stay above
-constexpr int64_t kMinTilePiece = 512;        // this many keys
+// How long the pieces are that it is cut into: a step fills the chip with some 384 workgroups, by pieces of 256 keys at
+// least, and then with up to 1024, by pieces of 1024 at least: more pieces even the load out, but each writes its rows in 32
+// bits and the join reads them.  One piece length for all would be (us, 512 and 1024 keys) 21.4 and 30.8 for a chunk of 64 behind
+// 4000, 67.6 and 55.5 for one of 256 behind 8000; 512, 768 or 1536 workgroups instead of 1024: 163, 160, 161 for 152
+// (two chunks among decoding steps).
+constexpr int64_t kTileTarget = 1024;
+constexpr int64_t kTileFill = 384;
+constexpr int64_t kShortPiece = 256;
+constexpr int64_t kLongPiece = 1024;
 constexpr int64_t kHeadBlock = 8;             // KV heads side by side: one for each of the chip's eight dies, which have an L2 each
 
 uint64_t kvm_step_seal(const KvmStep &s);

@@ -394,7 +394,7 @@ template <typename T, int SRC, int DP, int RT> struct Rows {
                 p4[rt][s] = __builtin_convertvector(sc[rt][s], typename Elem<T>::V4);
             }
             l[rt] = l[rt] * alpha + sum;
-            if (__any(alpha != 1.0f)) {
+            if (sizeof(T) == 4 || __any(alpha != 1.0f)) {   // most tiles move no maximum; bound by the product in 32 bits
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) acc[rt][dt] *= alpha;
             }
