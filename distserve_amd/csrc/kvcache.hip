@@ -22,8 +22,16 @@ using namespace kvc;
 // ---- write and read back
 //
 // Pure data movement: a lane takes eight elements of a row, 8, 16 or 32 lanes a row (the power of two
-// that covers head_dim; lanes past it idle).  Both are bound by HBM.  Consecutive rows of a workgroup are
-// consecutive tokens of one head, which lie side by side in the pool (codes and, more so, their scale bytes).
+// that covers head_dim; lanes past it idle).  Consecutive rows of a workgroup are consecutive tokens of one
+// head, which lie side by side in the pool (codes and, more so, their scale bytes).
+//
+// Both are bound by HBM, and by the launch where there is little to move.  Measured: 16 prompts, 20 heads of 128 in
+// bf16 (392 MB read and written) 70.5 us, 5.6 TB/s; 12 prompts, 8 heads of 128 in bf16 written as codes 24.4 us and
+// read back 17.5 us (179 MB together); one token of 96 sequences, 32 heads of 128, 2.7 us.  Two or four rows a lane, several
+// heads a workgroup, or workgroups of one wave were slower by 2 to 10 %.
+//
+// Quantising: e is the smallest exponent with max|x| <= 448 * 2^e, code = e4m3(x / 2^e), rounded to nearest even (half a step,
+// 2^-4 of the value); the division is by a power of two and exact.
 
 struct MoveArgs {
     const int32_t *slots;       // write: the new tokens' cache slots; read: {first output row, tokens} of each table entry
@@ -205,6 +213,11 @@ __global__ __launch_bounds__(256) void kvm_read_kernel(const MoveArgs a)
 
 // ---- attention
 
+// Bound by reading K and V (the launch and the plan's first words where there are few).  Measured, kernel alone:
+// single tokens of 32 sequences of 64 .. 2048, 32 heads of 128 in fp16, 80 us, 5.6 TB/s; of 8 sequences of 8000 .. 48000, 8 KV
+// heads in bf16, 104 us, 6.5 TB/s; of 64 sequences over e4m3 codes, 58 us, 5.1 TB/s, where turning codes into values
+// (VALU) and LDS take as long as memory.
+//
 // A workgroup for few rows walks its share of the units of all (row tile, KV head) pairs: perhaps the end of
 // a pair, then whole ones, then the beginning of one.  The next piece's first K is under way while a piece's
 // rows are joined and written.
@@ -275,6 +288,9 @@ struct JoinArgs {
     Divider by_group;
 };
 
+// Bound by reading the partial rows: 4 to 5 us behind single tokens, 11.6 us where two chunks of 700 tokens were cut
+// (36 MB), of which some 2 us are the launch.
+//
 // The lanes of a row look at the pieces' maxima and sums side by side; then the pieces' rows are added up, a few
 // loads in flight at a time.
 template <typename T, int LANES>

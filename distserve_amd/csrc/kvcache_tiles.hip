@@ -9,6 +9,13 @@
 // straight into LDS (plain pools and packed rows) or through registers, where codes become values
 // (quantised pools).  A row's 16-byte chunks are swapped around by the row's number, so that the 16
 // rows of an operand read, and the four rows of a transposing read, fall into different banks.
+//
+// Bound by the matrix cores and the softmax's VALU work, which take turns: on a prompt of 8192 tokens, 64 query and 8
+// KV heads of 128 in bf16, the matrix cores are busy 51 % of the time and the VALU 50 %, LDS 27 %, without bank
+// conflicts; 1.08 ms, 1.02 PFLOP/s (a large library product reaches 1.14 on this card).  Two workgroups a CU cover for
+// each other; 64 rows a wave, one workgroup a CU, is 2.7 times slower, and raising a wave's priority around the products or
+// summing weights by dot products changes nothing.  Lengths 64 .. 2048 packed, 32 heads: 0.36 ms, 0.67 PFLOP/s
+// (masked halves of tiles are computed and short prompts leave tiles part empty).
 #include "kv_internal.h"
 #include "kvcache_slow.h"
 #include "kvcache_tiles.h"
