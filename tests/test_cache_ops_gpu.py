@@ -1,4 +1,5 @@
 """The cache operators against their definition in 64 bits (cache_reference), on the GPU."""
+import gc
 import math
 import random
 
@@ -13,6 +14,15 @@ pytestmark = pytest.mark.gpu
 
 TYPES = [torch.float16, torch.bfloat16, torch.float32]
 CANARY = 0x5B
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _memory_goes_back():
+    """Large allocations are not left cached: later tests count on small ones of their own."""
+    yield
+    gc.collect()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
 
 
 def say(*what):
