@@ -331,8 +331,8 @@ __global__ __launch_bounds__(256) void kvm_join_kernel(const JoinArgs a)
     V4 *o = (V4 *)(a.out + (uint64_t)(j.q_start + token) * a.out_token + (uint64_t)((uint32_t)j.head * a.group + g) * a.out_head +
                    d * sizeof(T));
     const float inverse = 1.0f / sum;
-    o[0] = __builtin_convertvector(x * inverse, V4);
-    o[1] = __builtin_convertvector(y * inverse, V4);
+    o[0] = output4<T>(x * inverse);
+    o[1] = output4<T>(y * inverse);
 }
 
 // --------------------------------------------------------------------------- host

@@ -7,6 +7,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <type_traits>
 
 namespace kvc {
@@ -90,6 +91,21 @@ __device__ inline uint32_t saturated(uint32_t w)
     if ((w & 0x7fffu) == 0x7c00u) w -= 1;
     if ((w & 0x7fff0000u) == 0x7c000000u) w -= 0x10000u;
     return w;
+}
+
+// An output row's numbers in T's range.  A mean of fp16 numbers is in it, but weights that were rounded to fp16 for the product
+// (2^-11 of each at most) may carry it past the largest one, and from 2^-12 past it on it would round to an infinity: it is
+// the largest number then.  What V's infinities and NaN have made stays.
+template <typename T> __device__ inline float in_range(float x)
+{
+    if constexpr (std::is_same<T, _Float16>::value) return fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x;
+    return x;
+}
+template <typename T> __device__ inline typename Elem<T>::V4 output4(f32x4 x)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = in_range<T>(x[i]);
+    return __builtin_convertvector(x, typename Elem<T>::V4);
 }
 
 // Two elements of T in a word (one of float) as floats.

@@ -493,8 +493,8 @@ template <typename T, int SRC, int DP, int RT> struct Rows {
                                    d * sizeof(T));
                     const float inverse = 1.0f / sum;
                     if (live) {
-                        o[0] = __builtin_convertvector(x * inverse, V4);
-                        o[1] = __builtin_convertvector(y * inverse, V4);
+                        o[0] = output4<T>(x * inverse);
+                        o[1] = output4<T>(y * inverse);
                     }
                 }
             }

@@ -121,7 +121,7 @@ __device__ __forceinline__ void attend_slow(const AttnArgs &a, const RowWork w, 
             const int d = lane + 64 * i;
             if (d >= D) continue;
             if (w.part_row >= 0) a.part_acc[(uint64_t)(w.part_row + r) * D + d] = acc[i];
-            else *(T *)(dst + d * sizeof(T)) = (T)(acc[i] / l);
+            else *(T *)(dst + d * sizeof(T)) = (T)in_range<T>(acc[i] / l);
         }
         if (w.part_row >= 0 && lane == 0) *(f32x2 *)(a.part_ml + (uint64_t)(w.part_row + r) * 2) = f32x2{m, l};
     }

@@ -359,7 +359,7 @@ template <typename T, int SRC, int DP> struct TileKernel {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const f32x4 x = {acc[dt][4 * i], acc[dt][4 * i + 1], acc[dt][4 * i + 2], acc[dt][4 * i + 3]};
-                *(V4 *)(mine + col * kRow + ((4 * dt + i) ^ swizzle_out(col)) * 16 + half * 8) = __builtin_convertvector(x * inverse, V4);
+                *(V4 *)(mine + col * kRow + ((4 * dt + i) ^ swizzle_out(col)) * 16 + half * 8) = output4<T>(x * inverse);
             }
 #pragma unroll
         for (int j = 0; j < 2 * kLoads; ++j) {

@@ -1,0 +1,90 @@
+"""The cache operators at the edges of their types and arguments, on the GPU."""
+import gc
+import math
+
+import pytest
+import torch
+
+import cache_reference as ref
+from distserve_amd import paged_attention, plan_step, read_kv, write_kv
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float16, torch.bfloat16, torch.float32]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _memory_goes_back():
+    """Large allocations are not left cached: later tests count on small ones of their own."""
+    yield
+    gc.collect()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+
+
+def say(*what):
+    print(*what, flush=True)
+
+
+# first tokens, new tokens: one piece of the kernel for few rows, several that are joined, and the same of the one for many
+STEPS = {"row": (299, 1), "rows-joined": (5000, 2), "tile": (260, 40), "tiles-joined": (6000, 130)}
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("step", list(STEPS))
+@pytest.mark.parametrize("fmt", ["plain", "e4m3"])
+@pytest.mark.parametrize("every", [16, 1 << 30])
+def test_values_at_fp16s_largest_stay_numbers(step, fmt, d, every):
+    """Every value is fp16's largest, so every mean of them is.  The weights (1 for the first of every so many keys, just
+    above the middle of two fp16 numbers for the others) round up by nearly 2^-11 of themselves, and a mean that is
+    past 65520 by that would round to an infinity."""
+    say("largest", step, fmt, d, every)
+    first, new = STEPS[step]
+    n, block = first + new, 16
+    pages = -(-n // block)
+    weight = 0.5 + 1.05 * 2.0 ** -12
+    shape = (pages, 1, 1, block, d)
+    if fmt == "plain":
+        kc, vc = (torch.zeros(shape, dtype=torch.float16) for _ in range(2))
+        kc[..., 0] = -1.0
+        kc[0::max(1, every // 16), 0, 0, 0, 0] = 0.0
+        vc[..., ::2], vc[..., 1::2] = 65504.0, -65504.0
+    else:
+        kc, vc = (torch.zeros(*shape[:-1], d + 1, dtype=torch.uint8) for _ in range(2))
+        flat_k, flat_v = (x.view(pages, block * (d + 1)) for x in (kc, vc))
+        flat_k[:, 0:block * d:d] = 0xb8                   # -1
+        flat_k[0::max(1, every // 16), 0] = 0
+        flat_k[:, block * d:] = 127
+        flat_v[:, 0:block * d:2], flat_v[:, 1:block * d:2] = 0x7e, 0xfe      # 448 * 2^8, held as 65504
+        flat_v[:, block * d:] = 127 + 8
+    kc, vc = kc.cuda(), vc.cuda()
+    plan = plan_step(kc, [new], [first], [list(range(pages))], 1, torch.float16)
+    q = torch.zeros(new, 1, d, dtype=torch.float16, device="cuda")
+    q[..., 0] = 1.0
+    out = paged_attention(plan, 0, q, kc, vc, scale=-math.log(weight)).cpu().double()
+    # weights off by 2^-11 of themselves at most, and one rounding of the result
+    assert (out[..., ::2] - 65504.0).abs().max() <= 2 * 2.0 ** -11 * 65504.0
+    assert (out[..., 1::2] + 65504.0).abs().max() <= 2 * 2.0 ** -11 * 65504.0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quantising_the_smallest_numbers(dtype):
+    """Rows whose scale is 2^-126 or near it: codes times the scale are subnormal numbers of 32 bits."""
+    say("smallest", dtype)
+    d = 64
+    g = torch.Generator().manual_seed(3)
+    x = torch.empty(32, 1, d)
+    for i in range(32):                                  # largest magnitudes of about 2^-114 - i
+        x[i] = torch.randn(d, generator=g) * 2.0 ** (-114 - i)
+    x[30, 0] = torch.arange(64) * 2.0 ** -136            # multiples of half the smallest code's value
+    x[31, 0] = torch.arange(64) * 2.0 ** -133
+    x = x.to(dtype)
+    kc, vc = (torch.zeros(2, 1, 1, 16, d + 1, dtype=torch.uint8, device="cuda") for _ in range(2))
+    plan = plan_step(kc, [32], [0], [[1, 0]], 1, dtype)
+    write_kv(plan, 0, x.cuda(), x.cuda(), kc, vc)
+    k, v = read_kv(plan, 0, kc, vc)
+    want, e = ref.quantise(x)
+    assert e.min() == -126
+    for got in (k, v):
+        bad = (got.cpu().double() != want.to(dtype).double()).view(32, d)
+        assert not bad.any(), [(i, x[i, 0][bad[i]][:3].tolist(), got.cpu()[i, 0][bad[i]][:3].tolist()) for i in range(32) if bad[i].any()]
