@@ -14,6 +14,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <limits>
 
 namespace {
 
@@ -627,8 +628,9 @@ int attend(const KvmStep *step, const int32_t *words, AttnArgs a, int format, co
     a.by_block = divider(a.block_size ? a.block_size : 1);
     a.by_heads = divider(a.heads);
     a.by_group = divider(a.group);
-    // a negative scale turns q's signs over; a scale of zero is a tiny one, which keeps masked scores at -infinity
-    a.scale_log2 = fmaxf(fabsf(scale) * 1.44269504088896340736f, 1.2e-38f);
+    // a negative scale turns q's signs over; a scale of zero is the smallest one, which keeps masked scores at -infinity and makes
+    // no more than 2^-21 of the largest ones
+    a.scale_log2 = fmaxf(fabsf(scale) * 1.44269504088896340736f, std::numeric_limits<float>::denorm_min());
     a.q_sign = scale >= 0 ? 0u : size == 4 ? 0x80000000u : 0x80008000u;
     a.part_acc = (float *)workspace;
     a.part_ml = a.part_acc + step->part_rows * step->head_dim;

@@ -88,3 +88,26 @@ def test_quantising_the_smallest_numbers(dtype):
     for got in (k, v):
         bad = (got.cpu().double() != want.to(dtype).double()).view(32, d)
         assert not bad.any(), [(i, x[i, 0][bad[i]][:3].tolist(), got.cpu()[i, 0][bad[i]][:3].tolist()) for i in range(32) if bad[i].any()]
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_scale_of_zero_or_next_to_it_over_large_scores(dtype, new):
+    """Scores of +-1.6e37: nothing of them is left under a scale of 0 or of 2^-149."""
+    d, first = 16, 300
+    n = first + new
+    k = torch.full((n, 1, d), 1e18, dtype=dtype)
+    k[::2] = -1e18
+    v = torch.zeros(n, 1, d, dtype=dtype)
+    v[::2] = 1.0
+    q = torch.full((new, 1, d), 1e18, dtype=dtype)
+    kc, vc = (torch.zeros(-(-n // 16), 1, 1, 16, d, dtype=dtype, device="cuda") for _ in range(2))
+    table = [list(range(kc.shape[0]))]
+    whole = plan_step(kc, [n], [0], table, 1)
+    write_kv(whole, 0, k.cuda(), v.cuda(), kc, vc)
+    plan = plan_step(kc, [new], [first], table, 1)
+    for scale in (0.0, 2.0 ** -149, -2.0 ** -149):
+        say("scale", dtype, new, scale)
+        out = paged_attention(plan, 0, q.cuda(), kc, vc, scale=scale)
+        want, tol = ref.attention(q, k, v, first, scale, dtype)
+        assert ((out.cpu().double() - want).abs() <= tol).all(), scale
