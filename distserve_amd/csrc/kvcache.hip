@@ -598,7 +598,8 @@ template <typename T> int launch_join(const JoinArgs &a, uint32_t num_joins, int
 int attend(const KvmStep *step, const int32_t *words, AttnArgs a, int format, const KvmRows *q, const KvmRows *out,
            float scale, void *workspace, int64_t workspace_bytes, int device, hipStream_t stream)
 {
-    if (!std::isfinite(scale)) return refuse(KVM_EINVAL, "scale is not a finite number");
+    const float scale_log2 = fabsf(scale) * 1.44269504088896340736f;
+    if (!std::isfinite(scale_log2)) return refuse(KVM_EINVAL, "scale is not a finite number, or not one in powers of two (2.3e38 and more)");
     KV_TRY(check_rows(q, "q", step->num_tokens, step->num_heads, step, device));
     KV_TRY(check_rows(out, "out", step->num_tokens, step->num_heads, step, device));
     KV_TRY(check_apart(out, "out", step->num_tokens, step->num_heads, step->head_dim));
@@ -630,7 +631,7 @@ int attend(const KvmStep *step, const int32_t *words, AttnArgs a, int format, co
     a.by_group = divider(a.group);
     // a negative scale turns q's signs over; a scale of zero is the smallest one, which keeps masked scores at -infinity and makes
     // no more than 2^-21 of the largest ones
-    a.scale_log2 = fmaxf(fabsf(scale) * 1.44269504088896340736f, std::numeric_limits<float>::denorm_min());
+    a.scale_log2 = fmaxf(scale_log2, std::numeric_limits<float>::denorm_min());
     a.q_sign = scale >= 0 ? 0u : size == 4 ? 0x80000000u : 0x80008000u;
     a.part_acc = (float *)workspace;
     a.part_ml = a.part_acc + step->part_rows * step->head_dim;

@@ -1,0 +1,48 @@
+"""What the cache operators' entry points make of arguments at the edge of what they take, without a GPU."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from distserve_amd import cabi
+
+NO_GPU = pytest.mark.skipif(torch.cuda.is_available(),
+                            reason="the addresses are made up: only for a machine where nothing can be launched")
+
+K, V, Q, O, S, W, X = (i << 24 for i in range(1, 8))       # made-up addresses, 16 MiB apart
+POOL = 4 * 2 * 2 * 16 * 64 * 2
+
+
+def a_step(new=3, first=0, **kwargs):
+    args = dict(num_blocks=4, block_size=16, num_heads=8, num_kv_heads=2, head_dim=64, dtype=cabi.KVM_F16)
+    args.update(kwargs)
+    step, words = cabi.plan_step([first], [new], [list(range(-(-(first + new) // args["block_size"])))], **args)
+    step.device = 0                                        # the caller vouches for extents: no question to the runtime
+    return step
+
+
+def pools(**change):
+    args = dict(k=K, v=V, num_blocks=4, num_layers=2, layer=0, num_kv_heads=2, block_size=16, head_dim=64,
+                dtype=cabi.KVM_F16, format=cabi.KVM_CACHE_PLAIN, extent=POOL)
+    args.update(change)
+    return cabi.KvmCache(**args)
+
+
+def rows(at, token, head=64, extent=1 << 20):
+    return cabi.KvmRows(at, token, head, extent)
+
+
+def refused(code, text, call, *args):
+    with pytest.raises(cabi.KvmError, match=text) as e:
+        call(*args)
+    assert e.value.code == code, e.value
+
+
+@NO_GPU
+def test_scales_that_are_no_number_in_powers_of_two_are_refused():
+    step = a_step()
+    q, k, v, out = rows(Q, 512), rows(S, 128), rows(S + 4096, 128), rows(O, 512)
+    for scale in (3.0e38, -3.0e38, math.inf, math.nan):
+        refused(cabi.KVM_EINVAL, "scale", cabi.paged_attention, step, W, pools(), q, out, scale)
+        refused(cabi.KVM_EINVAL, "scale", cabi.prompt_attention, step, W, q, k, v, out, scale)
