@@ -423,7 +423,11 @@ int check_cache(const KvmStep *step, const KvmCache *c, int device, Layer *out)
     out->row_bytes = (uint32_t)(coded ? c->head_dim : c->head_dim * type_bytes(c->dtype));
     out->codes = (uint32_t)(c->block_size * c->head_dim);
     out->head_stride = (uint64_t)c->block_size * (out->row_bytes + (coded ? 1 : 0));
-    out->block_stride = out->head_stride * (uint64_t)(c->num_kv_heads * c->num_layers);
+    // (2^26 bytes of a slab, 2^20 heads and 2^31 slots at most, but any number of layers)
+    const unsigned __int128 all = (unsigned __int128)(out->head_stride * (uint64_t)c->num_kv_heads) * (uint64_t)c->num_layers;
+    if (all > (uint64_t)INT64_MAX || all * (uint64_t)c->num_blocks > (uint64_t)INT64_MAX)
+        return refuse(KVM_ERANGE, "a pool of %lld layers is too large", (long long)c->num_layers);
+    out->block_stride = (uint64_t)all;
     const uint64_t bytes = out->block_stride * (uint64_t)c->num_blocks;
     KV_TRY(check_memory(step, c->k, bytes, c->extent, "the K pool", &device));
     KV_TRY(check_memory(step, c->v, bytes, c->extent, "the V pool", &device));
@@ -445,7 +449,8 @@ int check_rows(const KvmRows *r, const char *what, int64_t tokens, int64_t heads
     const int64_t size = type_bytes(step->dtype);
     if (!r || !r->ptr) return refuse(KVM_EINVAL, "%s is null", what);
     if (r->token_stride < 0 || r->head_stride < 0) return refuse(KVM_EINVAL, "%s has a negative stride", what);
-    if ((uintptr_t)r->ptr % 16 != 0 || r->token_stride * size % 16 != 0 || r->head_stride * size % 16 != 0)
+    if ((uintptr_t)r->ptr % 16 != 0 || (uint64_t)r->token_stride * (uint64_t)size % 16 != 0 ||
+        (uint64_t)r->head_stride * (uint64_t)size % 16 != 0)
         return refuse(KVM_EINVAL, "%s: rows must start at multiples of 16 bytes (strides %lld and %lld elements)", what,
                       (long long)r->token_stride, (long long)r->head_stride);
     const unsigned __int128 need = reach(r, tokens, heads, step->head_dim) * (uint64_t)size;

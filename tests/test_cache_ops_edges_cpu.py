@@ -46,3 +46,18 @@ def test_scales_that_are_no_number_in_powers_of_two_are_refused():
     for scale in (3.0e38, -3.0e38, math.inf, math.nan):
         refused(cabi.KVM_EINVAL, "scale", cabi.paged_attention, step, W, pools(), q, out, scale)
         refused(cabi.KVM_EINVAL, "scale", cabi.prompt_attention, step, W, q, k, v, out, scale)
+
+
+@NO_GPU
+def test_sizes_whose_product_passes_64_bits_are_refused():
+    step = a_step()
+    q, k, v, out = rows(Q, 512), rows(S, 128), rows(S + 4096, 128), rows(O, 512)
+    for layers, layer in ((1 << 52, 1 << 50), (1 << 62, 3), ((1 << 63) - 1, 1 << 61), (1 << 50, 0)):
+        bad = pools(num_layers=layers, layer=layer, extent=(1 << 63) - 1)
+        refused(cabi.KVM_ERANGE, "pool", cabi.write_kv, step, W, bad, k, v)
+        refused(cabi.KVM_ERANGE, "pool", cabi.read_kv, step, W, bad, rows(O, 128), rows(O + 4096, 128))
+        refused(cabi.KVM_ERANGE, "pool", cabi.paged_attention, step, W, bad, q, out, 1.0)
+    # strides that are multiples of 2^64 bytes
+    for stride in (1 << 62, 3 << 61, (1 << 63) - 8):
+        refused(cabi.KVM_ERANGE, "too large", cabi.write_kv, step, W, pools(), rows(S, stride), v)
+        refused(cabi.KVM_ERANGE, "too large", cabi.write_kv, step, W, pools(), k, rows(S, 128, stride))
