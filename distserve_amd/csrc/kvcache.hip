@@ -500,6 +500,13 @@ int check_clear(const KvmRows *out, int64_t out_heads, const KvmRows *in, int64_
     return refuse(KVM_EINVAL, "%s share memory", what);
 }
 
+// The same for rows (their whole reach) and a stretch of memory: the plan's words, a workspace.
+int check_clear_of(const KvmRows *rows, int64_t tokens, int64_t heads, const KvmStep *step, const void *p, uint64_t bytes, const char *what)
+{
+    const uint64_t need = (uint64_t)reach(rows, tokens, heads, step->head_dim) * (uint64_t)type_bytes(step->dtype);
+    return disjoint(rows->ptr, need, p, bytes) ? KVM_OK : refuse(KVM_EINVAL, "%s share memory", what);
+}
+
 // The same for rows and whole pools.
 int check_clear_of_pools(const KvmRows *rows, int64_t tokens, int64_t heads, const KvmStep *step, const KvmCache *c, const Layer &layer,
                          const char *what)
@@ -615,7 +622,12 @@ int attend(const KvmStep *step, const int32_t *words, AttnArgs a, int format, co
             return refuse(KVM_EINVAL, "the workspace has %lld bytes, %lld (16-byte aligned) are needed",
                           (long long)(workspace ? workspace_bytes : 0), (long long)need);
         KV_TRY(check_memory(step, workspace, (uint64_t)need, workspace_bytes, "the workspace", &device));
+        KV_TRY(check_clear_of(q, step->num_tokens, step->num_heads, step, workspace, (uint64_t)need, "q and the workspace"));
+        KV_TRY(check_clear_of(out, step->num_tokens, step->num_heads, step, workspace, (uint64_t)need, "out and the workspace"));
+        if (!disjoint(words, (uint64_t)step->words * 4, workspace, (uint64_t)need))
+            return refuse(KVM_EINVAL, "the plan's words and the workspace share memory");
     }
+    KV_TRY(check_clear_of(out, step->num_tokens, step->num_heads, step, words, (uint64_t)step->words * 4, "out and the plan's words"));
     const uint64_t tile_groups = (uint64_t)(step->num_tile_items * std::min(step->num_kv_heads, kHeadBlock));
     if (tile_groups > kMaxGroups || (uint64_t)step->num_joins * 16 > kMaxGroups)
         return refuse(KVM_EINVAL, "too many rows for one launch");
@@ -691,6 +703,8 @@ int kvm_write_kv(const KvmStep *step, const int32_t *words, const KvmCache *cach
     KV_TRY(check_clear_of_pools(v, step->num_tokens, step->num_kv_heads, step, cache, layer, "v"));
     const uint64_t pool = layer.block_stride * (uint64_t)cache->num_blocks;
     if (!disjoint(cache->k, pool, cache->v, pool)) return refuse(KVM_EINVAL, "the K pool and the V pool share memory");
+    if (!disjoint(cache->k, pool, words, (uint64_t)step->words * 4) || !disjoint(cache->v, pool, words, (uint64_t)step->words * 4))
+        return refuse(KVM_EINVAL, "a pool and the plan's words share memory");
     if (step->num_tokens * step->num_kv_heads > INT32_MAX) return refuse(KVM_EINVAL, "too many rows for one launch");
     const uint64_t size = (uint64_t)type_bytes(step->dtype);
     MoveArgs a = {};
@@ -738,6 +752,9 @@ int kvm_read_kv(const KvmStep *step, const int32_t *words, const KvmCache *cache
     KV_TRY(check_clear(k_out, step->num_kv_heads, v_out, step->num_kv_heads, step->num_kv_tokens, step, "k_out and v_out"));
     KV_TRY(check_clear_of_pools(k_out, step->num_kv_tokens, step->num_kv_heads, step, cache, layer, "k_out"));
     KV_TRY(check_clear_of_pools(v_out, step->num_kv_tokens, step->num_kv_heads, step, cache, layer, "v_out"));
+    for (const KvmRows *r : {k_out, v_out})
+        KV_TRY(check_clear_of(r, step->num_kv_tokens, step->num_kv_heads, step, words, (uint64_t)step->words * 4,
+                              r == k_out ? "k_out and the plan's words" : "v_out and the plan's words"));
     if (step->num_pages * step->num_kv_heads > INT32_MAX) return refuse(KVM_EINVAL, "too many blocks for one launch");
     const uint64_t size = (uint64_t)type_bytes(step->dtype);
     MoveArgs a = {};
@@ -780,6 +797,9 @@ int kvm_paged_attention(const KvmStep *step, const int32_t *words, const KvmCach
     KV_TRY(check_cache(step, cache, device, &layer));
     KV_TRY(check_rows(out, "out", step->num_tokens, step->num_heads, step, device));
     KV_TRY(check_clear_of_pools(out, step->num_tokens, step->num_heads, step, cache, layer, "out"));
+    const uint64_t pool = layer.block_stride * (uint64_t)cache->num_blocks, scratch = (uint64_t)kvm_attention_workspace(step);
+    if (scratch > 0 && workspace && (!disjoint(workspace, scratch, cache->k, pool) || !disjoint(workspace, scratch, cache->v, pool)))
+        return refuse(KVM_EINVAL, "the workspace and a pool share memory");
     AttnArgs a = {};
     a.k = layer.k;
     a.v = layer.v;
@@ -808,6 +828,11 @@ int kvm_prompt_attention(const KvmStep *step, const int32_t *words, const KvmRow
     KV_TRY(check_rows(out, "out", step->num_tokens, step->num_heads, step, device));
     KV_TRY(check_clear(out, step->num_heads, k, step->num_kv_heads, step->num_tokens, step, "out and k"));
     KV_TRY(check_clear(out, step->num_heads, v, step->num_kv_heads, step->num_tokens, step, "out and v"));
+    const uint64_t scratch = (uint64_t)kvm_attention_workspace(step);
+    if (scratch > 0 && workspace) {
+        KV_TRY(check_clear_of(k, step->num_tokens, step->num_kv_heads, step, workspace, scratch, "k and the workspace"));
+        KV_TRY(check_clear_of(v, step->num_tokens, step->num_kv_heads, step, workspace, scratch, "v and the workspace"));
+    }
     AttnArgs a = {};
     a.k = (const char *)k->ptr;
     a.v = (const char *)v->ptr;

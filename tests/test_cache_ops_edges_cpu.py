@@ -61,3 +61,35 @@ def test_sizes_whose_product_passes_64_bits_are_refused():
     for stride in (1 << 62, 3 << 61, (1 << 63) - 8):
         refused(cabi.KVM_ERANGE, "too large", cabi.write_kv, step, W, pools(), rows(S, stride), v)
         refused(cabi.KVM_ERANGE, "too large", cabi.write_kv, step, W, pools(), k, rows(S, 128, stride))
+
+
+@NO_GPU
+def test_outputs_on_the_workspace_or_the_plan_are_refused():
+    step = a_step(1, 16 * 200, num_blocks=256)             # a long sequence: its keys are cut into pieces
+    need = cabi.attention_workspace(step)
+    assert need > 0
+    pool = dict(num_blocks=256, extent=64 * POOL)
+    words = step.words * 4
+    at = X + (1 << 24)                                     # workspace
+    q, out = rows(Q, 512), rows(O, 512)
+    for where in (at, at + need - 16, at - 16):
+        refused(cabi.KVM_EINVAL, "share memory", cabi.paged_attention, step, W, pools(**pool), q, rows(where, 512), 1.0, at, need)
+        refused(cabi.KVM_EINVAL, "share memory", cabi.paged_attention, step, W, pools(**pool), rows(where, 512), out, 1.0, at, need)
+    for where in (W - 16, W, W + words - 4 & ~15):
+        refused(cabi.KVM_EINVAL, "share memory", cabi.paged_attention, step, W, pools(**pool), q, rows(where, 512), 1.0, at, need)
+        refused(cabi.KVM_EINVAL, "share memory", cabi.paged_attention, step, W, pools(**pool), q, out, 1.0, where, need)
+    # the workspace on the pools
+    for where in (K, K + 64 * POOL - 16, V - 16):
+        refused(cabi.KVM_EINVAL, "share memory", cabi.paged_attention, step, W, pools(**pool), q, out, 1.0, where, need)
+    prompt = a_step(2000, num_blocks=256, num_kv_heads=8, dtype=cabi.KVM_F32)
+    need = cabi.attention_workspace(prompt)
+    assert need > 0
+    far = 1 << 40                                          # rows of 512 * 4 bytes, apart from each other
+    q, k, v, out = (cabi.KvmRows(far + (i << 28), 512, 64, 1 << 28) for i in range(4))
+    for where in (k.ptr, v.ptr + 4096, q.ptr + 2000 * 2048 - 16):
+        refused(cabi.KVM_EINVAL, "share memory", cabi.prompt_attention, prompt, W, q, k, v, out, 1.0, where, need)
+    refused(cabi.KVM_EINVAL, "share memory", cabi.prompt_attention, prompt, W, q, k, v, rows(W, 512, 64, 1 << 28), 1.0, far >> 1, need)
+    step = a_step()
+    refused(cabi.KVM_EINVAL, "share memory", cabi.write_kv, step, K + 4096, pools(), rows(S, 128), rows(S + 4096, 128))
+    refused(cabi.KVM_EINVAL, "share memory", cabi.read_kv, step, W, pools(), rows(W, 128), rows(O, 128))
+    refused(cabi.KVM_EINVAL, "share memory", cabi.read_kv, step, W, pools(), rows(O, 128), rows(W, 128))
