@@ -14,6 +14,7 @@
 #include <c10/hip/HIPStream.h>
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/custom_class.h>
 #include <torch/library.h>
@@ -22,6 +23,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <set>
@@ -132,9 +134,15 @@ struct StepPlan : torch::CustomClassHolder {
 
 typedef c10::intrusive_ptr<StepPlan> Plan;
 
-void no_grad(const at::Tensor &t, const char *op)
+// Nothing that a call reads or writes may be part of a derivative, backward or forward: it would be dropped without a word.
+void no_gradients(std::initializer_list<const at::Tensor *> tensors, const char *op)
 {
-    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), op, " has no gradient: call it under torch.no_grad()");
+    const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    for (const at::Tensor *t : tensors) {
+        if (!t) continue;
+        TORCH_CHECK(!(backward && t->requires_grad()), op, " has no gradient: call it under torch.no_grad()");
+        TORCH_CHECK(!(forward && t->_fw_grad(0).defined()), op, " has no gradient: a tensor has a forward-mode tangent");
+    }
 }
 
 // Bytes from the tensor's first element to the end of its storage.
@@ -144,7 +152,6 @@ int64_t extent(const at::Tensor &t) { return (int64_t)t.storage().nbytes() - t.s
 KvmRows rows(const Plan &plan, const at::Tensor &t, int64_t tokens, int64_t heads, const char *op, const char *name)
 {
     const KvmStep &s = plan->step;
-    no_grad(t, op);
     TORCH_CHECK(t.is_cuda(), op, ": ", name, " must live on the GPU");
     TORCH_CHECK(t.device() == plan->words.device(), op, ": ", name, " is on ", t.device(), ", the plan on ", plan->words.device());
     TORCH_CHECK(t.scalar_type() == plan->dtype, op, ": ", name, " is ", t.scalar_type(), ", the plan is for ", plan->dtype);
@@ -177,6 +184,7 @@ KvmCache cache(const Plan &plan, int64_t layer, const at::Tensor &k, const at::T
 void write_kv(const Plan &plan, int64_t layer, const at::Tensor &k, const at::Tensor &v, const at::Tensor &k_cache,
               const at::Tensor &v_cache)
 {
+    no_gradients({&k, &v, &k_cache, &v_cache}, "write_kv");
     void *stream;
     const int32_t *words = plan->use(k_cache, "write_kv", &stream);
     const KvmCache c = cache(plan, layer, k_cache, v_cache, "write_kv");
@@ -188,6 +196,7 @@ void write_kv(const Plan &plan, int64_t layer, const at::Tensor &k, const at::Te
 
 std::tuple<at::Tensor, at::Tensor> read_kv(const Plan &plan, int64_t layer, const at::Tensor &k_cache, const at::Tensor &v_cache)
 {
+    no_gradients({&k_cache, &v_cache}, "read_kv");
     void *stream;
     const int32_t *words = plan->use(k_cache, "read_kv", &stream);
     const KvmCache c = cache(plan, layer, k_cache, v_cache, "read_kv");
@@ -229,6 +238,7 @@ at::Tensor paged_attention(const Plan &plan, int64_t layer, const at::Tensor &q,
                            const at::Tensor &v_cache, std::optional<double> scale, const std::optional<at::Tensor> &out)
 {
     const char *op = "paged_attention";
+    no_gradients({&q, &k_cache, &v_cache, out.has_value() ? &*out : nullptr}, op);
     void *stream;
     const int32_t *words = plan->use(k_cache, op, &stream);
     const KvmCache c = cache(plan, layer, k_cache, v_cache, op);
@@ -248,6 +258,7 @@ at::Tensor prompt_attention(const Plan &plan, const at::Tensor &q, const at::Ten
                             std::optional<double> scale, const std::optional<at::Tensor> &out)
 {
     const char *op = "prompt_attention";
+    no_gradients({&q, &k, &v, out.has_value() ? &*out : nullptr}, op);
     void *stream;
     const int32_t *words = plan->use(q, op, &stream);
     const KvmStep &s = plan->step;

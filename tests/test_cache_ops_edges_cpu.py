@@ -93,3 +93,35 @@ def test_outputs_on_the_workspace_or_the_plan_are_refused():
     refused(cabi.KVM_EINVAL, "share memory", cabi.write_kv, step, K + 4096, pools(), rows(S, 128), rows(S + 4096, 128))
     refused(cabi.KVM_EINVAL, "share memory", cabi.read_kv, step, W, pools(), rows(W, 128), rows(O, 128))
     refused(cabi.KVM_EINVAL, "share memory", cabi.read_kv, step, W, pools(), rows(O, 128), rows(W, 128))
+
+
+def test_tensors_with_gradients_are_refused_wherever_they_stand():
+    """Rows, outputs and pools that require a gradient, and any of them with a forward-mode tangent."""
+    import distserve_amd
+    from torch.autograd import forward_ad
+
+    plan = distserve_amd.StepPlan([0], [3], [1], [1], 4, 16, 4, 2, 64, 5, False, -1)      # a plan to look at, without a GPU
+    pool = torch.zeros(4, 1, 2, 16, 64, dtype=torch.float16)
+    row, q = torch.zeros(3, 2, 64, dtype=torch.float16), torch.zeros(3, 4, 64, dtype=torch.float16)
+    calls = [
+        (lambda *t: distserve_amd.write_kv(plan, 0, *t), [row, row, pool, pool]),
+        (lambda *t: distserve_amd.read_kv(plan, 0, *t), [pool, pool]),
+        (lambda *t: distserve_amd.paged_attention(plan, 0, *t[:3], out=t[3]), [q, pool, pool, q]),
+        (lambda *t: distserve_amd.prompt_attention(plan, *t[:3], out=t[3]), [q, row, row, q]),
+    ]
+    ops = torch.ops.kvcache_ops
+    calls += [
+        (lambda *t: ops.write_kv(plan, 0, *t), [row, row, pool, pool]),
+        (lambda *t: ops.paged_attention(plan, 0, *t[:3], None, t[3]), [q, pool, pool, q]),
+    ]
+    for call, tensors in calls:
+        for i in range(len(tensors)):
+            wanted = [t.clone().requires_grad_() if i == j else t for j, t in enumerate(tensors)]
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call(*wanted)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="without a GPU"):       # as far as a machine without one gets
+                call(*wanted)
+            with forward_ad.dual_level():
+                dual = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(tensors)]
+                with pytest.raises(RuntimeError, match="no gradient"):
+                    call(*dual)
