@@ -304,8 +304,9 @@ KVM_TORCH_LIBRARY(KVM_CACHE_NS, m)
     m.def("write_kv(" KVM_PLAN ", int layer, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache) -> ()", write_kv);
     m.def("read_kv(" KVM_PLAN ", int layer, Tensor k_cache, Tensor v_cache) -> (Tensor, Tensor)", read_kv);
     m.def("paged_attention(" KVM_PLAN ", int layer, Tensor q, Tensor k_cache, Tensor v_cache, float? scale=None, "
-          "Tensor? out=None) -> Tensor",
+          "Tensor(a!)? out=None) -> Tensor(a!)",
           paged_attention);
-    m.def("prompt_attention(" KVM_PLAN ", Tensor q, Tensor k, Tensor v, float? scale=None, Tensor? out=None) -> Tensor",
+    m.def("prompt_attention(" KVM_PLAN ", Tensor q, Tensor k, Tensor v, float? scale=None, Tensor(a!)? out=None) -> "
+          "Tensor(a!)",
           prompt_attention);
 }

@@ -125,3 +125,21 @@ def test_tensors_with_gradients_are_refused_wherever_they_stand():
                 dual = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(tensors)]
                 with pytest.raises(RuntimeError, match="no gradient"):
                     call(*dual)
+
+
+@pytest.mark.parametrize("name", ["paged_attention", "prompt_attention"])
+@pytest.mark.parametrize("space", ["kvcache_ops", "kvmove_kvcache_ops"])
+def test_the_attention_ops_schemas_say_that_out_is_written_and_returned(space, name):
+    import os
+
+    import distserve_amd
+
+    if space != "kvcache_ops":
+        torch.ops.load_library(os.path.join(os.path.dirname(distserve_amd.TORCH_LIB_PATH), "libkvmove_torch_alt.so"))
+    schema = getattr(getattr(torch.ops, space), name).default._schema
+    out = schema.arguments[-1]
+    assert out.name == "out" and out.default_value is None and schema.is_mutable
+    assert out.alias_info is not None and out.alias_info.is_write
+    back = schema.returns[0].alias_info
+    assert back is not None and back.is_write and back.after_set == out.alias_info.before_set
+    assert [a.name for a in schema.arguments if a.alias_info is not None] == ["out"]
