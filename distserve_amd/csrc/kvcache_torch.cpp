@@ -145,6 +145,14 @@ void no_gradients(std::initializer_list<const at::Tensor *> tensors, const char 
     }
 }
 
+// A written tensor's version goes up, as after torch's own operators that write in place: a backward pass that has kept
+// what was there before is an error then instead of a wrong gradient.  (Tensors made in inference mode have no version.)
+void written(std::initializer_list<const at::Tensor *> tensors)
+{
+    for (const at::Tensor *t : tensors)
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // Bytes from the tensor's first element to the end of its storage.
 int64_t extent(const at::Tensor &t) { return (int64_t)t.storage().nbytes() - t.storage_offset() * (int64_t)t.element_size(); }
 
@@ -192,6 +200,7 @@ void write_kv(const Plan &plan, int64_t layer, const at::Tensor &k, const at::Te
     const KvmRows kr = rows(plan, k, s.num_tokens, s.num_kv_heads, "write_kv", "k"),
                   vr = rows(plan, v, s.num_tokens, s.num_kv_heads, "write_kv", "v");
     check(kvm_write_kv(&s, words, &c, &kr, &vr, stream), "write_kv");
+    written({&k_cache, &v_cache});
 }
 
 std::tuple<at::Tensor, at::Tensor> read_kv(const Plan &plan, int64_t layer, const at::Tensor &k_cache, const at::Tensor &v_cache)
@@ -251,6 +260,7 @@ at::Tensor paged_attention(const Plan &plan, int64_t layer, const at::Tensor &q,
     check(kvm_paged_attention(&s, words, &c, &qr, &orows, scale_of(plan, scale), w.defined() ? w.data_ptr() : nullptr,
                               w.defined() ? w.numel() : 0, stream),
           op);
+    if (out.has_value()) written({&o});
     return o;
 }
 
@@ -271,6 +281,7 @@ at::Tensor prompt_attention(const Plan &plan, const at::Tensor &q, const at::Ten
     check(kvm_prompt_attention(&s, words, &qr, &kr, &vr, &orows, scale_of(plan, scale), w.defined() ? w.data_ptr() : nullptr,
                                w.defined() ? w.numel() : 0, stream),
           op);
+    if (out.has_value()) written({&o});
     return o;
 }
 

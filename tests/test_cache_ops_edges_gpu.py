@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import cache_reference as ref
-from distserve_amd import paged_attention, plan_step, read_kv, write_kv
+from distserve_amd import paged_attention, plan_prompt, plan_step, prompt_attention, read_kv, write_kv
 
 pytestmark = pytest.mark.gpu
 
@@ -111,3 +111,35 @@ def test_a_scale_of_zero_or_next_to_it_over_large_scores(dtype, new):
         out = paged_attention(plan, 0, q.cuda(), kc, vc, scale=scale)
         want, tol = ref.attention(q, k, v, first, scale, dtype)
         assert ((out.cpu().double() - want).abs() <= tol).all(), scale
+
+
+@pytest.mark.parametrize("through", ["functions", "ops"])
+def test_writes_raise_the_versions_of_what_they_write(through):
+    """A backward pass that kept a pool or an output from before the call is refused, not wrong."""
+    ops = torch.ops.kvcache_ops
+    pools = [torch.zeros(2, 1, 2, 16, 64, device="cuda") for _ in range(2)]
+    row, q = torch.ones(3, 2, 64, device="cuda"), torch.ones(3, 4, 64, device="cuda")
+    out = torch.zeros_like(q)
+    plan, prompt = plan_step(pools[0], [3], [0], [[1]], 4), plan_prompt([3], 4, 2, 64, torch.float32)
+    w = torch.ones((), device="cuda", requires_grad=True)
+    kept = [(w * t).sum() for t in (*pools, out)]
+    with torch.no_grad():
+        if through == "functions":
+            write_kv(plan, 0, row, row, *pools)
+            assert paged_attention(plan, 0, q, *pools, out=out) is not None
+            versions = [t._version for t in (row, q, out, *pools)]
+            prompt_attention(prompt, q, row, row, out=out)
+        else:
+            ops.write_kv(plan, 0, row, row, *pools)
+            ops.paged_attention(plan, 0, q, *pools, None, out)
+            versions = [t._version for t in (row, q, out, *pools)]
+            ops.prompt_attention(prompt, q, row, row, None, out)
+    assert versions[:2] == [0, 0] and [t._version for t in (row, q, out, *pools)] == [0, 0, versions[2] + 1, *versions[3:]]
+    for y in kept:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():                           # tensors without a version stay usable, inside and out
+        made = [torch.zeros_like(p) for p in pools]
+        write_kv(plan, 0, row, row, *made)
+    write_kv(plan, 0, row, row, *made)
+    assert torch.equal(paged_attention(plan, 0, q, *made), q)
