@@ -4,10 +4,11 @@
 // and reduced to pointers, sizes and strides; the current HIP stream of their device is handed to the
 // C ABI.  A nonzero return code becomes a RuntimeError carrying kvm_last_error().
 //
-// The plan's words are copied to the device on a stream of their own and the copy is waited
-// for, so a plan is complete when its constructor returns: it can be used on any stream
-// afterwards, and in a captured graph (a graph holds the plan's address, so the plan has to
-// live as long as the graph).
+// The plan's words go from pinned memory to the device on the current stream, and nobody waits for them on the host: that
+// stream is behind whatever the program has given it, a stream of its own for the copies often behind another one (small
+// copies are kernels, on a hardware queue that several streams share).  Calls on other streams wait there for the
+// copy's event.  Only a call that is captured waits on the host, once, because the graph may run anywhere (a graph holds
+// the plan's address, so the plan has to live as long as the graph).
 #include "kvmove.h"
 
 #include <c10/hip/HIPGuard.h>
@@ -23,8 +24,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <initializer_list>
-#include <map>
 #include <mutex>
 #include <set>
 #include <vector>
@@ -46,23 +47,23 @@ int32_t type_code(at::ScalarType t)
     }
 }
 
-// The stream that a device's plans are copied on.
-c10::hip::HIPStream copy_stream(c10::DeviceIndex device)
-{
-    static std::mutex mu;
-    static std::map<c10::DeviceIndex, c10::hip::HIPStream> streams;
-    std::lock_guard<std::mutex> lock(mu);
-    auto it = streams.find(device);
-    if (it == streams.end()) it = streams.emplace(device, c10::hip::getStreamFromPool(false, device)).first;
-    return it->second;
-}
+// While another thread captures a graph, the calls that a plan's copy needs are allowed to this one (and while this thread
+// does, waiting for such a copy is).
+struct BesideCaptures {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    BesideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+    ~BesideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+};
 
 struct StepPlan : torch::CustomClassHolder {
     KvmStep step;
     at::Tensor words;
     c10::ScalarType dtype;
     std::mutex mu;
-    std::set<hipStream_t> seen;   // streams the allocator has been told of
+    std::set<hipStream_t> seen;   // streams the allocator has been told of, and made to wait for the words
+    hipStream_t made_on = nullptr;
+    hipEvent_t copied = nullptr;  // of the words, on made_on
+    bool complete = false;        // the copy is known to have ended
 
     StepPlan(std::vector<int64_t> first_token, std::vector<int64_t> new_tokens, std::vector<int64_t> table,
              std::vector<int64_t> table_len, int64_t num_blocks, int64_t block_size, int64_t num_heads,
@@ -96,24 +97,33 @@ struct StepPlan : torch::CustomClassHolder {
               "StepPlan");
         if (device < 0) return;   // a plan to look at, without a GPU
         const c10::hip::HIPGuard guard((c10::DeviceIndex)device);
-        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-        TORCH_CHECK(hipStreamIsCapturing(c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream(), &capture) == hipSuccess &&
-                        capture == hipStreamCaptureStatusNone,
-                    "StepPlan: make the plan before the graph capture that uses it");
-        const c10::hip::HIPStream stream = copy_stream((c10::DeviceIndex)device);
-        {
-            // allocated on the copy stream, so that the memory is free there; users are announced by use()
-            const c10::hip::HIPStreamGuard on(stream);
-            words = at::empty({std::max<int64_t>(step.words, 4)}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, device));
-        }
-        TORCH_CHECK(hipMemcpyAsync(words.data_ptr(), host.data(), (size_t)step.words * 4, hipMemcpyHostToDevice, stream.stream()) == hipSuccess &&
-                        hipStreamSynchronize(stream.stream()) == hipSuccess,
-                    "StepPlan: copying the plan to the device failed");
+        made_on = c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream();
+        TORCH_CHECK(!captures(made_on), "StepPlan: make the plan before the graph capture that uses it");
+        const BesideCaptures allowed;
+        const int64_t room = std::max<int64_t>(step.words, 4);
+        const at::Tensor staged = at::empty({room}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
+        std::memcpy(staged.data_ptr(), host.data(), (size_t)step.words * 4);
+        words = at::empty({room}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, device));
+        words.copy_(staged, /*non_blocking=*/true);      // torch keeps the pinned memory until the copy has ended
+        TORCH_CHECK(hipEventCreateWithFlags(&copied, hipEventDisableTiming) == hipSuccess &&
+                        hipEventRecord(copied, made_on) == hipSuccess,
+                    "StepPlan: no event for the plan's copy");
         step.device = device;    // the ops below check where their tensors are and how far they reach
     }
 
-    // The words for a call on `device`'s current stream; the allocator is told of the stream, so that the
-    // words' memory is not handed out again before the stream's work is done.
+    ~StepPlan() override
+    {
+        if (copied) (void)hipEventDestroy(copied);
+    }
+
+    static bool captures(hipStream_t stream)
+    {
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        return hipStreamIsCapturing(stream, &status) != hipSuccess || status != hipStreamCaptureStatusNone;
+    }
+
+    // The words for a call on `device`'s current stream, which comes after their copy; the allocator is told of the stream, so
+    // that the words' memory is not handed out again before the stream's work is done.
     const int32_t *use(const at::Tensor &like, const char *op, void **stream)
     {
         TORCH_CHECK(words.defined(), op, ": the plan was made without a GPU");
@@ -123,8 +133,23 @@ struct StepPlan : torch::CustomClassHolder {
         *stream = (void *)s.stream();
         {
             std::lock_guard<std::mutex> lock(mu);
-            if (seen.insert(s.stream()).second)
+            if (!complete) {
+                // asked until it is: where the GPU is far behind the host, the host has the time
+                const BesideCaptures allowed;
+                complete = hipEventQuery(copied) == hipSuccess;
+                if (!complete) {
+                    (void)hipGetLastError();     // that it is not ready is no error
+                    if (captures(s.stream())) {
+                        TORCH_CHECK(hipEventSynchronize(copied) == hipSuccess, op, ": waiting for the plan's copy failed");
+                        complete = true;
+                    }
+                }
+            }
+            if (seen.insert(s.stream()).second) {
                 words.record_stream(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device).unwrap());
+                if (!complete && s.stream() != made_on)
+                    TORCH_CHECK(hipStreamWaitEvent(s.stream(), copied, 0) == hipSuccess, op, ": waiting for the plan's copy failed");
+            }
         }
         return words.data_ptr<int32_t>();
     }

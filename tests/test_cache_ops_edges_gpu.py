@@ -143,3 +143,94 @@ def test_writes_raise_the_versions_of_what_they_write(through):
         write_kv(plan, 0, row, row, *made)
     write_kv(plan, 0, row, row, *made)
     assert torch.equal(paged_attention(plan, 0, q, *made), q)
+
+
+def long_step(seqs, seed=0):
+    """Pools of random values and a plan of one new token for each of some sequences, in scattered blocks."""
+    g = torch.Generator().manual_seed(seed)
+    pools = [torch.randn(seqs * 20, 1, 2, 16, 64, generator=g).half().cuda() for _ in range(2)]
+    table = torch.randperm(seqs * 20, generator=g).view(seqs, 20).tolist()
+    make = lambda: plan_step(pools[0], [1] * seqs, [319 - i % 50 for i in range(seqs)], table, 4)
+    q = torch.randn(seqs, 4, 64, generator=g).half().cuda()
+    return pools, make, q
+
+
+def test_plans_are_made_whichever_stream_is_busy():
+    """The stream that the plan is for, and torch's pool of 32 once around and more, each busy in its turn."""
+    pools, make, q = long_step(8)
+    want = paged_attention(make(), 0, q, *pools)
+    torch.cuda.synchronize()
+    for i in range(41):
+        stream = torch.cuda.Stream() if i else torch.cuda.current_stream()
+        done = torch.cuda.Event()
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(100_000_000)                 # some 40 ms, a plan takes 0.1
+        done.record(stream)
+        plan = make()
+        assert not done.query(), f"the plan waited for stream {i}"
+        out = paged_attention(plan, 0, q, *pools)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+
+
+def test_plans_made_on_a_busy_stream_are_used_on_others_and_in_graphs():
+    """The words are still on their way when the plan is used: on another stream, in a capture, and when it is gone."""
+    pools, make, q = long_step(8, 2)
+    want = paged_attention(make(), 0, q, *pools)
+    others = [long_step(8, 3 + i) for i in range(4)]
+    torch.cuda.synchronize()
+    for turn in range(6):
+        busy, user = torch.cuda.Stream(), torch.cuda.Stream()
+        with torch.cuda.stream(busy):
+            torch.cuda._sleep(25_000_000)
+            plan = make()
+        if turn % 2:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=user):
+                out = paged_attention(plan, 0, q, *pools)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(3):
+                    graph.replay()
+        else:
+            with torch.cuda.stream(user):
+                out = paged_attention(plan, 0, q, *pools)
+                torch.cuda._sleep(100_000_000)
+                again = paged_attention(plan, 0, q, *pools)
+            del plan
+            # plans of the same size, made on the stream whose memory the words are: theirs is not to be given away while a
+            # call of another stream is yet to run
+            with torch.cuda.stream(busy):
+                kept = [m() for _, m, _ in others for _ in range(4)]
+            torch.cuda.synchronize()
+            assert torch.equal(again, want) and len(kept) == 16
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), turn
+
+
+def test_plans_are_made_while_another_thread_captures():
+    import threading
+
+    pools, make, q = long_step(8, 1)
+    first = make()
+    want = paged_attention(first, 0, q, *pools)
+    made, errors = [], []
+
+    def plan(turn):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream() if turn % 2 else torch.cuda.default_stream()):
+                made.append(make())
+        except Exception as e:                             # told in the assertion below
+            errors.append(e)
+
+    for turn in range(40):                                 # the capture streams go round torch's pool
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph, stream=side):
+            thread = threading.Thread(target=plan, args=(turn,))
+            thread.start()
+            thread.join()
+            out = paged_attention(first, 0, q, *pools)
+        assert not errors, errors
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert torch.equal(paged_attention(made[-1], 0, q, *pools), want), turn
