@@ -34,7 +34,8 @@ class CacheConfig:
 
     ``cache_dtype`` (not in the reference): "auto" keeps K and V in the model's type, "e4m3" as
     8-bit codes with a power-of-two scale for each token and head (``head_dim + 1`` bytes).  Both
-    instances of a deployment must use the same: migration moves blocks as they are."""
+    instances of a deployment must use the same: migration moves blocks as they are, and a worker
+    refuses the handles of pools of the other kind."""
 
     def __init__(self, block_size: int, max_num_blocks_per_req: int,
                  gpu_memory_utilization: float = 0.9, cpu_swap_space: int = 0, cache_dtype: str = "auto"):

@@ -57,7 +57,9 @@ void register_ipc_mem_handle_from(int64_t context_instance, std::vector<int64_t>
                                   std::vector<int64_t> context_parallel_config,
                                   std::vector<int64_t> decoding_parallel_config)
 {
-    TORCH_CHECK(k_handle.size() == KVM_HANDLE_WORDS && v_handle.size() == KVM_HANDLE_WORDS,
+    // (a quantised pool's handle has one more, for the workers to compare: the words before it say where the pool is)
+    const size_t words = k_handle.size();
+    TORCH_CHECK((words == KVM_HANDLE_WORDS || words == KVM_HANDLE_WORDS + 1) && v_handle.size() == words,
                 "register_ipc_mem_handle: a memory handle has ", KVM_HANDLE_WORDS, " words");
     TORCH_CHECK(context_parallel_config.size() == 4 && decoding_parallel_config.size() == 4,
                 "register_ipc_mem_handle: parallel configs are [tp_size, tp_rank, pp_size, pp_rank]");

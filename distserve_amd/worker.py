@@ -23,7 +23,7 @@ from typing import Callable, Dict, List, Optional, Tuple
 
 import torch
 
-from distserve_amd import cache_ops
+from distserve_amd import cabi, cache_ops
 from distserve_amd.config import CacheConfig, ModelConfig, ParallelConfig
 from distserve_amd.request import Request
 from distserve_amd.streams import side_streams
@@ -160,12 +160,14 @@ class Worker:
 
     def init_kvcache_and_swap(self, num_gpu_blocks: int, num_cpu_blocks: int) -> Tuple[MemoryHandle, MemoryHandle]:
         """Allocate the K/V pools on HBM and the pinned K/V swap pools on the host; return the
-        memory handles of the two HBM pools (reference worker.py:101-134)."""
+        memory handles of the two HBM pools (reference worker.py:101-134).  A quantised pool's
+        handle has a word more, which says so."""
         self.k_cache, self.v_cache = (self._new_pool(num_gpu_blocks, on_host=False) for _ in range(2))
         self.k_swap, self.v_swap = (self._new_pool(num_cpu_blocks, on_host=True) for _ in range(2))
         torch.cuda.synchronize()
         export = torch.ops.block_migration_ops.get_ipc_mem_handle
-        return export(self.k_cache), export(self.v_cache)
+        mark = [cabi.KVM_CACHE_E4M3] if self.cache_is_quantized else []
+        return export(self.k_cache) + mark, export(self.v_cache) + mark
 
     def _get_block_size_in_bytes(self, block_size: int, model_config: ModelConfig,
                                  parallel_config: ParallelConfig) -> int:
@@ -235,20 +237,34 @@ class Worker:
 
     # ---- migration
 
+    def _check_pool_format(self, pair: Tuple[MemoryHandle, MemoryHandle], pp_rank: int, tp_rank: int) -> None:
+        names = {cabi.KVM_CACHE_PLAIN: "plain", cabi.KVM_CACHE_E4M3: "e4m3"}
+        ours = cabi.KVM_CACHE_E4M3 if self.cache_is_quantized else cabi.KVM_CACHE_PLAIN
+        for handle in pair:
+            mark = list(handle[cabi.KVM_HANDLE_WORDS:]) or [cabi.KVM_CACHE_PLAIN]
+            if mark != [ours]:
+                theirs = names.get(mark[0], "unknown") if len(mark) == 1 else "unknown"
+                raise RuntimeError(f"context rank ({pp_rank}, {tp_rank})'s pools are {theirs}, this worker's are {names[ours]}: "
+                                   "both instances must use the same cache_dtype")
+
     def register_kvcache_mem_handles(self, context_parallel_config: ParallelConfig,
                                      kvcache_ipc_mem_handles: List[List[Tuple[MemoryHandle, MemoryHandle]]],
                                      context_instance: int = 0) -> None:
         """Bind every context rank's pools, ``handles[pp_rank][tp_rank] = (k, v)``
         (reference worker.py:229-248).  The handles may come from another process: they are
         plain lists of ints.  ``context_instance`` (not in the reference, where a decoding
-        worker serves one context instance) keeps several instances' pools apart."""
+        worker serves one context instance) keeps several instances' pools apart.  Pools of
+        another ``cache_dtype`` than this worker's are refused before any is bound: blocks move as they are."""
+        for pp_rank, stage_handles in enumerate(kvcache_ipc_mem_handles):
+            for tp_rank, pair in enumerate(stage_handles):
+                self._check_pool_format(pair, pp_rank, tp_rank)
         for pp_rank, stage_handles in enumerate(kvcache_ipc_mem_handles):
             for tp_rank, (k_handle, v_handle) in enumerate(stage_handles):
                 rank_config = copy.deepcopy(context_parallel_config)
                 rank_config.pipeline_parallel_rank = pp_rank
                 rank_config.tensor_parallel_rank = tp_rank
                 torch.ops.block_migration_ops.register_ipc_mem_handle_from(
-                    context_instance, k_handle, v_handle,
+                    context_instance, list(k_handle[:cabi.KVM_HANDLE_WORDS]), list(v_handle[:cabi.KVM_HANDLE_WORDS]),
                     self.model_config.get_num_layers(), self.model_config.get_num_heads(),
                     rank_config.to_list(), self.parallel_config.to_list())
         torch.cuda.synchronize()

@@ -234,3 +234,18 @@ def test_plans_are_made_while_another_thread_captures():
         torch.cuda.synchronize()
         assert torch.equal(out, want)
         assert torch.equal(paged_attention(made[-1], 0, q, *pools), want), turn
+
+
+@pytest.mark.parametrize("ctx_dtype,dec_dtype", [("auto", "e4m3"), ("e4m3", "auto")])
+def test_instances_with_pools_of_different_kinds_are_not_bound(ctx_dtype, dec_dtype):
+    from distserve_amd import CacheConfig, ContextStageLLMEngine, DecodingStageLLMEngine, ModelConfig, ParallelConfig, cabi
+
+    cabi.reset()
+    model = ModelConfig.from_kv_shape(2, 8, 64, 4)
+    ctx = ContextStageLLMEngine(model, ParallelConfig(2, 0, 1, 0), CacheConfig(16, 64, cache_dtype=ctx_dtype))
+    dec = DecodingStageLLMEngine(model, ParallelConfig(), CacheConfig(16, 64, cache_dtype=dec_dtype))
+    ctx._init_kvcache(256, 0)                              # of 65 or 128 bytes a row: either divides the other's pool
+    dec._init_kvcache(65, 2)
+    with pytest.raises(RuntimeError, match="same cache_dtype"):
+        dec.register_kvcache_mem_handles(ctx.parallel_config, ctx.kv_cache_mem_handles)
+    cabi.reset()
