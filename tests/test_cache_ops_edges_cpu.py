@@ -143,3 +143,45 @@ def test_the_attention_ops_schemas_say_that_out_is_written_and_returned(space, n
     back = schema.returns[0].alias_info
     assert back is not None and back.is_write and back.after_set == out.alias_info.before_set
     assert [a.name for a in schema.arguments if a.alias_info is not None] == ["out"]
+
+
+@pytest.mark.parametrize("block", [16, 32, 8, 24, 1])
+@pytest.mark.parametrize("dtype", [cabi.KVM_F16, cabi.KVM_BF16, cabi.KVM_F32])
+def test_which_kernel_a_sequences_rows_go_to(dtype, block):
+    """More than 16 rows of 16 bits for a KV head go to the kernel for many rows, where blocks are whole sixteens; all
+    others to the one for few, two row tiles at a time if one of them has more than 16 and head_dim is 128 at most.
+    Either way every row's keys are covered once, from the first to its own."""
+    for heads, kv_heads, head_dim in ((1, 1, 64), (8, 8, 128), (12, 3, 64), (17, 1, 128), (16, 2, 256), (48, 2, 80)):
+        group = heads // kv_heads
+        news = sorted({n for rows in (1, 15, 16, 17, 23, 24, 31, 32, 33, 48, 129) for n in (rows // group, -(-rows // group)) if n})
+        for new in ([n] for n in news):
+            new = new + [1, 0, 2]
+            first = [100, 0, 7, 3000]
+            pages = [-(-(a + b) // block) for a, b in zip(first, new)]
+            at, table = 0, []
+            for p in pages:
+                table.append(list(range(at, at + p)))
+                at += p
+            step, words = cabi.plan_step(first, new, table, at + 1, block, heads, kv_heads, head_dim, dtype)
+            many = [dtype != cabi.KVM_F32 and n * group > 16 and block % 16 == 0 for n in new]
+            few_rows = [n * group for n, m in zip(new, many) if not m]
+            assert step.row_tiles == (2 if max(few_rows, default=0) > 16 and head_dim <= 128 else 1)
+            height = 16 * step.row_tiles
+            tiles = [tuple(words[step.row_tiles_at + 8 * i:step.row_tiles_at + 8 * i + 8]) for i in range(step.num_row_tiles)]
+            items = [tuple(words[step.tile_items_at + 12 * i:step.tile_items_at + 12 * i + 12]) for i in range(step.num_tile_items)]
+            want_tiles, starts = [], [sum(new[:s]) for s in range(len(new))]
+            for s, n in enumerate(new):
+                for r in range(0, 0 if many[s] else n * group, height):
+                    end = first[s] + (min(r + height, n * group) - 1) // group + 1
+                    want_tiles.append((starts[s], n * group, first[s], sum(pages[:s]), r, end, -(-end // 128)))
+            assert [t[:7] for t in tiles] == want_tiles
+            for s, n in enumerate(new):
+                mine = [i for i in items if i[0] == starts[s] and i[1] == n * group and n]
+                if not many[s]:
+                    assert not mine
+                    continue
+                for r in range(0, n * group, 128):
+                    for head0 in range(0, kv_heads, 8):
+                        cut = sorted((i[5], i[6]) for i in mine if i[4] == r and i[8] == head0)
+                        assert cut[0][0] == 0 and all(a[1] == b[0] for a, b in zip(cut, cut[1:]))
+                        assert cut[-1][1] == first[s] + (min(r + 128, n * group) - 1) // group + 1

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import cache_reference as ref
+from test_cache_ops_gpu import Case
 from distserve_amd import paged_attention, plan_prompt, plan_step, prompt_attention, read_kv, write_kv
 
 pytestmark = pytest.mark.gpu
@@ -249,3 +250,38 @@ def test_instances_with_pools_of_different_kinds_are_not_bound(ctx_dtype, dec_dt
     with pytest.raises(RuntimeError, match="same cache_dtype"):
         dec.register_kvcache_mem_handles(ctx.parallel_config, ctx.kv_cache_mem_handles)
     cabi.reset()
+
+
+# ---- chunks and prompts over blocks that are not multiples of 16: the kernel for few rows, two row tiles at a time
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("block", [8, 24])
+@pytest.mark.parametrize("hq,h,d", [(8, 2, 64), (4, 4, 96), (8, 1, 128), (4, 2, 256)])
+def test_chunks_over_other_block_sizes(dtype, block, hq, h, d):
+    say("chunks, blocks of", block, dtype, hq, h, d)
+    case = Case(dtype, "plain", hq, h, d, block, [0, 300, 77, 1500, 40], [70, 33, 1, 2, 0], seed=d + block)
+    case.check(case.attend(), fast=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("block", [8, 16])
+@pytest.mark.parametrize("hq,h,d", [(8, 2, 64), (4, 4, 80), (8, 1, 128), (2, 2, 256)])
+def test_prompts_under_a_plan_with_a_pool(dtype, block, hq, h, d):
+    """K and V are rows at hand; the plan is the step's, with the pool that they are written to."""
+    say("prompts, blocks of", block, dtype, hq, h, d)
+    lens = [1, 130, 0, 63, 17]
+    case = Case(dtype, "plain", hq, h, d, block, [0] * 5, lens, seed=d)
+    k, v = (torch.cat(parts).to(dtype) for parts in case.seqs)
+    case.check(prompt_attention(case.plan, case.q.cuda(), k.cuda(), v.cuda()), fast=True)
+    case.check(case.attend(), fast=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [15, 16, 17, 24, 32, 33])
+@pytest.mark.parametrize("fmt", ["plain", "e4m3"])
+def test_both_sides_of_the_border_between_the_kernels(dtype, rows, fmt):
+    """16 rows of a KV head (tokens and heads of its group) go to the kernel for few rows, 17 to the one for many."""
+    say("border", dtype, rows, fmt)
+    for hq, new in {(1, rows), (rows, 1)} | ({(3, rows // 3)} if rows % 3 == 0 else set()):
+        case = Case(dtype, fmt, 2 * hq, 2, 64, 16, [200, 0, 1000], [new, new, 1], seed=rows)
+        case.check(case.attend(), fast=True)
