@@ -285,3 +285,23 @@ def test_both_sides_of_the_border_between_the_kernels(dtype, rows, fmt):
     for hq, new in {(1, rows), (rows, 1)} | ({(3, rows // 3)} if rows % 3 == 0 else set()):
         case = Case(dtype, fmt, 2 * hq, 2, 64, 16, [200, 0, 1000], [new, new, 1], seed=rows)
         case.check(case.attend(), fast=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_code_under_every_scale(dtype):
+    """A quantised pool's values as its format defines them, rounded to the rows' type once (past fp16's largest: that)."""
+    say("codes", dtype)
+    d = 256
+    pool = torch.zeros(16, 1, 1, 16, d + 1, dtype=torch.uint8)
+    flat = pool.view(16, 16 * (d + 1))
+    flat[:, :16 * d] = torch.arange(256, dtype=torch.uint8).repeat(16)
+    flat[:, 16 * d:] = torch.arange(256, dtype=torch.uint8).view(16, 16)
+    want = ref.decode_pool(pool, d).view(256, d)[:255]
+    if dtype == torch.float16:
+        want = want.clamp(-65504.0, 65504.0)
+    want = want.to(dtype)
+    plan = plan_step(pool.cuda(), [1], [254], [list(range(16))], 1, dtype)
+    for got in read_kv(plan, 0, pool.cuda(), pool.cuda()):
+        got = got.cpu().view(255, d)
+        bad = ~((got == want) | (got.isnan() & want.isnan()))
+        assert not bad.any(), [(s - 127, hex(c), got[s, c].item(), want[s, c].item()) for s, c in bad.nonzero()[:8].tolist()]
