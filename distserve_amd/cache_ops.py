@@ -21,11 +21,19 @@ reads; the K and the V pool of a write must be two.  Such calls are refused.
 
 A pool is plain, ``[num_blocks, layers, kv_heads, block_size, head_dim]`` of the rows' type, or
 quantised: uint8 with last dimension ``head_dim + 1`` (``quantized_pool_shape``), e4m3 codes with a
-power-of-two scale for each token and head.  Migration and swap move both.
+power-of-two scale for each token and head.  Migration and swap move both.  Chunks and prompts are fastest where
+``block_size`` is a multiple of 16: over other blocks every row of a plan goes to the kernel for few rows
+(512 tokens behind thousands, 64 heads over 8: 1.5 ms instead of 0.35).
 
-Everything runs on the current stream of the tensors' device and returns without waiting.
+Everything, a plan's copy to the GPU too, runs on the current stream of the tensors' device and returns
+without waiting; a plan made on one stream can be used on any other, which then waits for its copy.
 Calls can be captured into a graph; the plan must have been made before the capture and live
-as long as the graph.  There are no gradients: a call on tensors that require one is refused.
+as long as the graph.  There are no gradients: a call on tensors that require one (rows, pools or ``out``),
+or that have a forward-mode tangent, is refused, and what a call writes has its version raised.
+
+Scores, softmax sums and accumulators are 32-bit.  The softmax weights of float16 and bfloat16 rows are rounded to
+the rows' type for the product with V, half a step of each, which adds about as much error as the
+rounding of the result does (relative to the definition, 2.9e-4 instead of 2.1e-4 in float16, 2.1e-3 instead of 1.6e-3 in bfloat16).
 """
 from __future__ import annotations
 

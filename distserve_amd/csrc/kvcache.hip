@@ -216,8 +216,9 @@ __global__ __launch_bounds__(256) void kvm_read_kernel(const MoveArgs a)
 
 // Bound by reading K and V (the launch and the plan's first words where there are few).  Measured, kernel alone:
 // single tokens of 32 sequences of 64 .. 2048, 32 heads of 128 in fp16, 80 us, 5.6 TB/s; of 8 sequences of 8000 .. 48000, 8 KV
-// heads in bf16, 104 us, 6.5 TB/s; of 64 sequences over e4m3 codes, 58 us, 5.1 TB/s, where turning codes into values
-// (VALU) and LDS take as long as memory.
+// heads in bf16, 104 us, 6.5 TB/s; of 64 sequences over e4m3 codes, 58 us, 5.1 TB/s, where LDS is busy 47 % of the time (39 % of
+// that with bank conflicts), VALU 37 %, and nothing is full.  In 32 bits, 32 sequences of 64 .. 2048, 32 heads, 173 us, 5.2 TB/s;
+// 64 sequences over codes 144 us; chunks of 512 behind thousands 69 TFLOP/s and packed prompts 58 (a library product: 154).
 //
 // A workgroup for few rows walks its share of the units of all (row tile, KV head) pairs: perhaps the end of
 // a pair, then whole ones, then the beginning of one.  The next piece's first K is under way while a piece's

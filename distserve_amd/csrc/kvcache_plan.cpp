@@ -182,14 +182,17 @@ try {
     // ---- attention work: row tiles, each over the keys its last row may see
     //
     // Sequences of many rows go to the tile kernel (16-bit types; its loads want 16 keys in one block),
-    // the others to the row kernel.
+    // the others to the row kernel.  (Chunks of 512 behind thousands, 64 heads over 8 of 128, fp16: 350 us over blocks of 16,
+    // 1516 us over blocks of 8.)
     auto in_tiles = [&](int64_t s) {
         return dtype != KVM_F32 && new_tokens[s] * group > kFewRows && (!cached || block_size % 16 == 0);
     };
     int64_t most_rows = 0;
     for (int64_t s = 0; s < num_seqs; ++s)
         if (!in_tiles(s)) most_rows = std::max(most_rows, new_tokens[s] * group);
-    // two 16-row tiles share the keys that a wave loads, where the registers hold their accumulators
+    // Two 16-row tiles share the keys that a wave loads, where the registers hold their accumulators.  The widest sequence decides for
+    // the step: 32 sequences of 1500, 32 heads over 8, all of one token or one of them of five, 77 and 125 us in fp32, 37 and 54 us in
+    // fp16 over blocks of 8.
     out.row_tiles = most_rows > 16 && head_dim <= 128 ? 2 : 1;
 
     // few rows: the keys of all (row tile, KV head) pairs in a row, dealt out evenly in units

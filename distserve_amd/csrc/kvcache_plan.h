@@ -45,8 +45,8 @@ constexpr int64_t kJoinWords = sizeof(KvJoin) / 4;
 
 constexpr int64_t kUnit = 128;                // keys the four waves of a workgroup for few rows take in one turn
 constexpr int64_t kCus = 256;
-// Up to here a sequence's rows go to the kernel for few rows.  16 sequences of 2048, 8 KV heads of 128, fp16, in us: 16 rows 31.8
-// there, 42.7 in the kernel for many; 24 rows 55.2 and 49.8; 32 heads of 1000 keys, 24 rows 79 and 56.
+// Up to here a sequence's rows go to the kernel for few rows.  16 sequences of 2048, 8 KV heads of 128, fp16, in us: 16 rows 31.6
+// there, 42.3 in the kernel for many; 24 rows 55.4 and 42.6; 32 heads of 1000 keys, 24 rows 80.7 and 56.1.
 constexpr int64_t kFewRows = 16;
 constexpr int64_t kTileRows = 128;            // of a workgroup of the kernel for many rows
 constexpr int64_t kTileStep = 64;             // keys of its tiles

@@ -14,8 +14,9 @@
 // KV heads of 128 in bf16, the matrix cores are busy 51 % of the time and the VALU 50 %, LDS 27 %, without bank
 // conflicts; 1.08 ms, 1.02 PFLOP/s (a large library product reaches 1.14 on this card).  Two workgroups a CU cover for
 // each other; 64 rows a wave, one workgroup a CU, is 2.7 times slower, and raising a wave's priority around the products or
-// summing weights by dot products changes nothing.  Lengths 64 .. 2048 packed, 32 heads: 0.36 ms, 0.67 PFLOP/s
-// (masked halves of tiles are computed and short prompts leave tiles part empty).
+// summing weights by dot products changes nothing.  Lengths 64 .. 2048 packed, 32 heads: 0.37 ms, 0.66 PFLOP/s,
+// of an item 13 tiles on average: masked and empty parts of tiles are 6 % of the work by waves and 18 % by workgroups, matrix cores are
+// busy 35 % and VALU 44 %; the rest is what an item does before its first product and after its last.
 #include "kv_internal.h"
 #include "kvcache_slow.h"
 #include "kvcache_tiles.h"

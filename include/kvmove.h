@@ -361,7 +361,8 @@ int kvm_read_kv(const KvmStep *step, const int32_t *words, const KvmCache *cache
 
 /* Bytes of device workspace kvm_paged_attention / kvm_prompt_attention want (may be 0); the
  * contents do not matter and nothing is kept in it between calls, but two calls in flight on
- * different streams (or two captured graphs that replay at the same time) need one each. */
+ * different streams (or two captured graphs that replay at the same time) need one each.  It
+ * must not lie on the rows, the pools or the plan's words (KVM_EINVAL). */
 int64_t kvm_attention_workspace(const KvmStep *step);
 
 /*
@@ -371,8 +372,12 @@ int64_t kvm_attention_workspace(const KvmStep *step);
  * The new tokens' K and V must be in the cache (kvm_write_kv before it on the stream).
  * Tokens behind the last sequence's in q and out are neither read nor written.  Cache slots
  * that no row may attend to (blocks' unused tails, later tokens) do not reach the result,
- * whatever they hold.  Sums, maxima and accumulators are 32-bit.
- * out may lie between q's rows in memory (slices of one wider row), not on them, nor in the pools.
+ * whatever they hold.  Scores, sums, maxima and accumulators are 32-bit; the weights of 16-bit
+ * rows are rounded to the rows' type for the product with V (half a step of each: 2^-11 of it for
+ * KVM_F16, 2^-8 for KVM_BF16), the results once more.  A KVM_F16 result of finite V that the weights'
+ * rounding carries past the largest number becomes that number.
+ * |scale| may be 2.3e38 at most.  out may lie between q's rows in memory (slices of one wider row),
+ * not on them, nor in the pools or on the plan's words.
  */
 int kvm_paged_attention(const KvmStep *step, const int32_t *words, const KvmCache *cache, const KvmRows *q,
                         const KvmRows *out, float scale, void *workspace, int64_t workspace_bytes, void *stream);
