@@ -4,11 +4,13 @@
 // and reduced to pointers, sizes and strides; the current HIP stream of their device is handed to the
 // C ABI.  A nonzero return code becomes a RuntimeError carrying kvm_last_error().
 //
-// The plan's words go from pinned memory to the device on the current stream, and nobody waits for them on the host: that
-// stream is behind whatever the program has given it, a stream of its own for the copies often behind another one (small
-// copies are kernels, on a hardware queue that several streams share).  Calls on other streams wait there for the
-// copy's event.  Only a call that is captured waits on the host, once, because the graph may run anywhere (a graph holds
+// The plan's words are copied to the device on the current stream, and nobody waits for them on the host: that stream is
+// behind whatever the program has given it, a stream of its own for the copies often behind another one (small copies are
+// kernels, on a hardware queue that several streams share).  Calls on other streams wait there for the copy's event.
+// Only a call that is captured waits on the host, once, because the graph may run anywhere (a graph holds
 // the plan's address, so the plan has to live as long as the graph).
+// The host looks at a word that the stream writes behind the copy: an event counts as captured while the stream it was recorded
+// on captures, however long ago that was, and to ask for it breaks the capture.
 #include "kvmove.h"
 
 #include <c10/hip/HIPGuard.h>
@@ -23,11 +25,13 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <chrono>
 #include <cmath>
 #include <cstring>
 #include <initializer_list>
 #include <mutex>
 #include <set>
+#include <thread>
 #include <vector>
 
 namespace {
@@ -47,12 +51,67 @@ int32_t type_code(at::ScalarType t)
     }
 }
 
-// While another thread captures a graph, the calls that a plan's copy needs are allowed to this one (and while this thread
-// does, waiting for such a copy is).
+// While another thread captures a graph, the calls that a plan's copy needs are allowed to this one.
 struct BesideCaptures {
     hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
     BesideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
     ~BesideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+};
+
+// A word of pinned memory that a stream writes a number of its own to.  It goes from plan to plan once that has happened.  (Nothing
+// here is ever destroyed: plans may be dropped after everything else.)
+class Mark {
+    struct Words {
+        std::mutex mu;
+        std::vector<uint32_t *> free;        // written, so nobody's
+        std::vector<Mark> dropped;           // of plans that were gone before the stream came to it
+        uint32_t last = 0;
+    };
+    static Words &words()
+    {
+        static Words *all = new Words;
+        return *all;
+    }
+    uint32_t *at = nullptr, number = 0;
+
+public:
+    bool reached() const { return __atomic_load_n(at, __ATOMIC_ACQUIRE) == number; }
+
+    // Behind what `stream` has now.
+    bool set(hipStream_t stream)
+    {
+        Words &w = words();
+        std::lock_guard<std::mutex> lock(w.mu);
+        for (size_t i = 0; i < w.dropped.size();) {
+            if (w.dropped[i].reached()) {
+                w.free.push_back(w.dropped[i].at);
+                w.dropped[i] = w.dropped.back();
+                w.dropped.pop_back();
+            } else {
+                ++i;
+            }
+        }
+        if (w.free.empty()) {
+            constexpr int kWords = 64, kApart = 16;     // a cache line each
+            uint32_t *more = nullptr;
+            if (hipHostMalloc((void **)&more, kWords * kApart * sizeof(uint32_t), hipHostMallocPortable | hipHostMallocCoherent) != hipSuccess) return false;
+            std::memset(more, 0, kWords * kApart * sizeof(uint32_t));
+            for (int i = 0; i < kWords; ++i) w.free.push_back(more + i * kApart);
+        }
+        if (++w.last == 0) ++w.last;                    // not what fresh words hold
+        if (hipStreamWriteValue32(stream, w.free.back(), w.last, 0) != hipSuccess) return false;
+        at = w.free.back();
+        number = w.last;
+        w.free.pop_back();
+        return true;
+    }
+    void drop()
+    {
+        if (!at) return;
+        std::lock_guard<std::mutex> lock(words().mu);
+        words().dropped.push_back(*this);
+        at = nullptr;
+    }
 };
 
 struct StepPlan : torch::CustomClassHolder {
@@ -62,7 +121,8 @@ struct StepPlan : torch::CustomClassHolder {
     std::mutex mu;
     std::set<hipStream_t> seen;   // streams the allocator has been told of, and made to wait for the words
     hipStream_t made_on = nullptr;
-    hipEvent_t copied = nullptr;  // of the words, on made_on
+    hipEvent_t copied = nullptr;  // behind the copy on made_on, as the mark
+    Mark mark;
     bool complete = false;        // the copy is known to have ended
 
     StepPlan(std::vector<int64_t> first_token, std::vector<int64_t> new_tokens, std::vector<int64_t> table,
@@ -100,19 +160,20 @@ struct StepPlan : torch::CustomClassHolder {
         made_on = c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream();
         TORCH_CHECK(!captures(made_on), "StepPlan: make the plan before the graph capture that uses it");
         const BesideCaptures allowed;
-        const int64_t room = std::max<int64_t>(step.words, 4);
-        const at::Tensor staged = at::empty({room}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
-        std::memcpy(staged.data_ptr(), host.data(), (size_t)step.words * 4);
-        words = at::empty({room}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, device));
-        words.copy_(staged, /*non_blocking=*/true);      // torch keeps the pinned memory until the copy has ended
-        TORCH_CHECK(hipEventCreateWithFlags(&copied, hipEventDisableTiming) == hipSuccess &&
-                        hipEventRecord(copied, made_on) == hipSuccess,
-                    "StepPlan: no event for the plan's copy");
+        words = at::empty({std::max<int64_t>(step.words, 4)}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, device));
+        // (from pageable memory: it has been read when the call returns)
+        bool ok = hipMemcpyAsync(words.data_ptr(), host.data(), (size_t)step.words * 4, hipMemcpyHostToDevice, made_on) == hipSuccess;
+        ok = ok && hipEventCreateWithFlags(&copied, hipEventDisableTiming) == hipSuccess && hipEventRecord(copied, made_on) == hipSuccess;
+        if (!ok || !mark.set(made_on)) {
+            if (copied) (void)hipEventDestroy(copied);
+            TORCH_CHECK(false, "StepPlan: copying the plan to the device failed");
+        }
         step.device = device;    // the ops below check where their tensors are and how far they reach
     }
 
     ~StepPlan() override
     {
+        mark.drop();
         if (copied) (void)hipEventDestroy(copied);
     }
 
@@ -120,6 +181,16 @@ struct StepPlan : torch::CustomClassHolder {
     {
         hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
         return hipStreamIsCapturing(stream, &status) != hipSuccess || status != hipStreamCaptureStatusNone;
+    }
+
+    // On the host, for what made_on was given before the copy.
+    void wait_for_words(const char *op)
+    {
+        const auto start = std::chrono::steady_clock::now();
+        while (!(complete = complete || mark.reached())) {
+            std::this_thread::sleep_for(std::chrono::microseconds(20));
+            TORCH_CHECK(std::chrono::steady_clock::now() - start < std::chrono::minutes(10), op, ": the plan's copy does not end");
+        }
     }
 
     // The words for a call on `device`'s current stream, which comes after their copy; the allocator is told of the stream, so
@@ -133,22 +204,15 @@ struct StepPlan : torch::CustomClassHolder {
         *stream = (void *)s.stream();
         {
             std::lock_guard<std::mutex> lock(mu);
-            if (!complete) {
-                // asked until it is: where the GPU is far behind the host, the host has the time
-                const BesideCaptures allowed;
-                complete = hipEventQuery(copied) == hipSuccess;
-                if (!complete) {
-                    (void)hipGetLastError();     // that it is not ready is no error
-                    if (captures(s.stream())) {
-                        TORCH_CHECK(hipEventSynchronize(copied) == hipSuccess, op, ": waiting for the plan's copy failed");
-                        complete = true;
-                    }
-                }
-            }
-            if (seen.insert(s.stream()).second) {
+            complete = complete || mark.reached();
+            if (!complete && captures(s.stream())) wait_for_words(op);   // the graph may run at any time on any stream
+            if (seen.count(s.stream()) == 0) {
                 words.record_stream(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device).unwrap());
-                if (!complete && s.stream() != made_on)
-                    TORCH_CHECK(hipStreamWaitEvent(s.stream(), copied, 0) == hipSuccess, op, ": waiting for the plan's copy failed");
+                if (!complete && s.stream() != made_on && hipStreamWaitEvent(s.stream(), copied, 0) != hipSuccess) {
+                    (void)hipGetLastError();     // made_on captures in another thread: the event cannot be had now
+                    wait_for_words(op);
+                }
+                seen.insert(s.stream());
             }
         }
         return words.data_ptr<int32_t>();

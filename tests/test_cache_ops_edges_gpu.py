@@ -305,3 +305,75 @@ def test_every_code_under_every_scale(dtype):
         got = got.cpu().view(255, d)
         bad = ~((got == want) | (got.isnan() & want.isnan()))
         assert not bad.any(), [(s - 127, hex(c), got[s, c].item(), want[s, c].item()) for s, c in bad.nonzero()[:8].tolist()]
+
+
+def test_a_capture_on_the_stream_that_still_copies_the_plan():
+    pools, make, q = long_step(8, 8)
+    want = paged_attention(make(), 0, q, *pools)
+    torch.cuda.synchronize()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(50_000_000)
+        plan = make()
+        graph.capture_begin()                              # without the wait for the GPU that torch.cuda.graph begins with
+        try:
+            out = paged_attention(plan, 0, q, *pools)
+        finally:
+            graph.capture_end()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_a_plan_is_used_while_the_stream_it_was_made_on_captures_elsewhere():
+    """One thread captures on the stream that a plan was made on, in the mode that lets other threads work; another uses that
+    plan and makes plans meanwhile."""
+    import threading
+
+    pools, make, q = long_step(8, 10)
+    want = paged_attention(make(), 0, q, *pools)
+    torch.cuda.synchronize()
+    for turn in range(4):
+        stream, graph, got, errors = torch.cuda.Stream(), torch.cuda.CUDAGraph(), [], []
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(25_000_000)
+            first, second = make(), make()
+
+        def work():
+            try:
+                with torch.cuda.stream(torch.cuda.Stream()):
+                    got.append(paged_attention(second, 0, q, *pools))
+                    got.append(paged_attention(make(), 0, q, *pools))
+            except Exception as e:                         # told in the assertion below
+                errors.append(e)
+
+        with torch.cuda.stream(stream):
+            graph.capture_begin(capture_error_mode="thread_local")
+            try:
+                thread = threading.Thread(target=work)
+                if turn % 2:                               # before the copy has ended, or after the captured call has waited for it
+                    thread.start()
+                    thread.join()
+                out = paged_attention(first, 0, q, *pools)
+                if turn % 2 == 0:
+                    thread.start()
+                    thread.join()
+            finally:
+                graph.capture_end()
+        assert not errors, errors
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and len(got) == 2 and all(torch.equal(g, want) for g in got), turn
+
+
+def test_plans_made_in_inference_mode_are_used_outside_of_it():
+    pools, make, q = long_step(4, 9)
+    want = paged_attention(make(), 0, q, *pools)
+    with torch.inference_mode():
+        plan = make()
+        inside = paged_attention(plan, 0, q, *pools)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        outside = paged_attention(plan, 0, q, *pools)
+    torch.cuda.synchronize()
+    assert torch.equal(inside, want) and torch.equal(outside, want)
