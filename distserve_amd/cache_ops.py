@@ -27,8 +27,8 @@ power-of-two scale for each token and head.  Migration and swap move both.  Chun
 
 Everything, a plan's copy to the GPU too, runs on the current stream of the tensors' device and returns
 without waiting; a plan made on one stream can be used on any other, which then waits for its copy.
-Calls can be captured into a graph; the plan must have been made before the capture and live
-as long as the graph.  There are no gradients: a call on tensors that require one (rows, pools or ``out``),
+Calls can be captured into a graph; the plan must have been made before the capture, and the graph keeps
+what it needs of it.  There are no gradients: a call on tensors that require one (rows, pools or ``out``),
 or that have a forward-mode tangent, is refused, and what a call writes has its version raised.
 
 Scores, softmax sums and accumulators are 32-bit.  The softmax weights of float16 and bfloat16 rows are rounded to

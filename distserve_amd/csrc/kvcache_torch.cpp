@@ -7,8 +7,7 @@
 // The plan's words are copied to the device on the current stream, and nobody waits for them on the host: that stream is
 // behind whatever the program has given it, a stream of its own for the copies often behind another one (small copies are
 // kernels, on a hardware queue that several streams share).  Calls on other streams wait there for the copy's event.
-// Only a call that is captured waits on the host, once, because the graph may run anywhere (a graph holds
-// the plan's address, so the plan has to live as long as the graph).
+// Only a call that is captured waits on the host, once, because the graph may run anywhere; and the graph keeps the words.
 // The host looks at a word that the stream writes behind the copy: an event counts as captured while the stream it was recorded
 // on captures, however long ago that was, and to ask for it breaks the capture.
 #include "kvmove.h"
@@ -51,7 +50,8 @@ int32_t type_code(at::ScalarType t)
     }
 }
 
-// While another thread captures a graph, the calls that a plan's copy needs are allowed to this one.
+// While another thread captures a graph, the calls that a plan's copy needs are allowed to this one (and while this thread
+// does, those that tie the words to the graph).
 struct BesideCaptures {
     hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
     BesideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
@@ -114,6 +114,33 @@ public:
     }
 };
 
+// Plans' words that a graph kept and has let go.  A graph tells that from wherever it is taken apart, where no call of the runtime
+// is allowed: the memory goes back when the next plan is made or dropped.  (Never destroyed: graphs may outlive everything.)
+struct LetGo {
+    std::mutex mu;
+    std::vector<at::Tensor *> words;
+    static LetGo &list()
+    {
+        static LetGo *all = new LetGo;
+        return *all;
+    }
+    static void by_graph(void *kept)
+    {
+        LetGo &all = list();
+        std::lock_guard<std::mutex> lock(all.mu);
+        all.words.push_back((at::Tensor *)kept);
+    }
+    static void give_back()
+    {
+        std::vector<at::Tensor *> gone;
+        {
+            std::lock_guard<std::mutex> lock(list().mu);
+            gone.swap(list().words);
+        }
+        for (at::Tensor *t : gone) delete t;
+    }
+};
+
 struct StepPlan : torch::CustomClassHolder {
     KvmStep step;
     at::Tensor words;
@@ -124,6 +151,7 @@ struct StepPlan : torch::CustomClassHolder {
     hipEvent_t copied = nullptr;  // behind the copy on made_on, as the mark
     Mark mark;
     bool complete = false;        // the copy is known to have ended
+    unsigned long long captured_by = 0;   // the last capture that keeps the words
 
     StepPlan(std::vector<int64_t> first_token, std::vector<int64_t> new_tokens, std::vector<int64_t> table,
              std::vector<int64_t> table_len, int64_t num_blocks, int64_t block_size, int64_t num_heads,
@@ -156,6 +184,7 @@ struct StepPlan : torch::CustomClassHolder {
                             quantized ? KVM_CACHE_E4M3 : KVM_CACHE_PLAIN, host.data(), (int64_t)host.size(), &step),
               "StepPlan");
         if (device < 0) return;   // a plan to look at, without a GPU
+        LetGo::give_back();
         const c10::hip::HIPGuard guard((c10::DeviceIndex)device);
         made_on = c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream();
         TORCH_CHECK(!captures(made_on), "StepPlan: make the plan before the graph capture that uses it");
@@ -175,6 +204,7 @@ struct StepPlan : torch::CustomClassHolder {
     {
         mark.drop();
         if (copied) (void)hipEventDestroy(copied);
+        if (words.defined()) LetGo::give_back();
     }
 
     static bool captures(hipStream_t stream)
@@ -193,6 +223,30 @@ struct StepPlan : torch::CustomClassHolder {
         }
     }
 
+    // A captured call: the graph may run at any time on any stream, so the words have to be there, and stay as long as the graph.
+    void keep_for_graph(hipStream_t stream, const char *op)
+    {
+        wait_for_words(op);
+        const BesideCaptures allowed;
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        unsigned long long id = 0;
+        hipGraph_t graph = nullptr;
+        TORCH_CHECK(hipStreamGetCaptureInfo_v2(stream, &status, &id, &graph, nullptr, nullptr) == hipSuccess && graph, op,
+                    ": no graph to capture into");
+        if (id == captured_by) return;
+        hipUserObject_t object = nullptr;
+        at::Tensor *kept = new at::Tensor(words);
+        if (hipUserObjectCreate(&object, kept, LetGo::by_graph, 1, hipUserObjectNoDestructorSync) != hipSuccess) {
+            delete kept;
+            TORCH_CHECK(false, op, ": the graph cannot keep the plan");
+        }
+        if (hipGraphRetainUserObject(graph, object, 1, hipGraphUserObjectMove) != hipSuccess) {
+            (void)hipUserObjectRelease(object, 1);
+            TORCH_CHECK(false, op, ": the graph cannot keep the plan");
+        }
+        captured_by = id;
+    }
+
     // The words for a call on `device`'s current stream, which comes after their copy; the allocator is told of the stream, so
     // that the words' memory is not handed out again before the stream's work is done.
     const int32_t *use(const at::Tensor &like, const char *op, void **stream)
@@ -205,7 +259,7 @@ struct StepPlan : torch::CustomClassHolder {
         {
             std::lock_guard<std::mutex> lock(mu);
             complete = complete || mark.reached();
-            if (!complete && captures(s.stream())) wait_for_words(op);   // the graph may run at any time on any stream
+            if (captures(s.stream())) keep_for_graph(s.stream(), op);
             if (seen.count(s.stream()) == 0) {
                 words.record_stream(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device).unwrap());
                 if (!complete && s.stream() != made_on && hipStreamWaitEvent(s.stream(), copied, 0) != hipSuccess) {

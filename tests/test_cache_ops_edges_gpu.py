@@ -377,3 +377,46 @@ def test_plans_made_in_inference_mode_are_used_outside_of_it():
         outside = paged_attention(plan, 0, q, *pools)
     torch.cuda.synchronize()
     assert torch.equal(inside, want) and torch.equal(outside, want)
+
+
+def test_graphs_keep_the_words_of_the_plans_they_were_captured_with():
+    """A plan dropped after the capture: its words stay as long as the graph does, and no longer."""
+    pools, make, q = long_step(8, 7)
+    want = paged_attention(make(), 0, q, *pools)
+    gc.collect()
+    torch.cuda.synchronize()
+    make()                                                 # (whatever earlier graphs let go is given back)
+    start = torch.cuda.memory_allocated()
+    plan = make()
+    size = torch.cuda.memory_allocated() - start
+    assert size > 0
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph in graphs:
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            outs.append([paged_attention(plan, 0, q, *pools) for _ in range(2)])
+    held = torch.cuda.memory_allocated()
+    del plan
+    gc.collect()
+    assert torch.cuda.memory_allocated() == held           # nothing below replays if this does not hold
+    junk = [torch.full((size // 4,), -1, dtype=torch.int32, device="cuda") for _ in range(16)]
+    for turn in range(3):
+        for i in range(2):
+            for out in outs[i]:
+                out.zero_()
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(out, want) for out in outs[i]), turn
+            assert torch.equal(paged_attention(make(), 0, q, *pools), want)
+    del junk
+    graphs.pop()
+    gc.collect()
+    make()
+    graphs[0].replay()                                     # the other graph's are still there
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for out in outs[0])
+    before = torch.cuda.memory_allocated()
+    del graph
+    graphs.clear()
+    gc.collect()
+    make()
+    assert torch.cuda.memory_allocated() <= before - size   # (a graph has a little of its own)
